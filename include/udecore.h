@@ -328,6 +328,79 @@ int ude_last_failures(ude_ctx* ctx, const int32_t* retcode_dev, int64_t N, int32
  * measured with HIP events on the context's stream (valid after the stream has been synchronised) */
 int ude_last_kernel_ms(ude_ctx* ctx, float* fwd_ms, float* bwd_ms);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * Training operators on device buffers: a gated feed-forward block with its pullback, the AdamW step over many tensors, the global
+ * gradient norm.  They replace nothing of the reference's scripts (their networks are Dense chains and their optimiser is ADAM:
+ * scenario_1.jl:62-64,111; highdim_pde/lambaem.jl:23-31): they are the layer and the optimiser step of larger networks, next to them.
+ * Every call enqueues on the context's stream, may be captured into a hipGraph and uses no memory but its arguments: the caller owns
+ * the workspace (its contents need not be kept between calls; calls that may run at the same time -- two streams, two captured graphs
+ * -- need one each).  Sizes and host-side arguments are baked into a captured call. */
+enum { UDE_DT_F64 = 0, UDE_DT_F32 = 1, UDE_DT_F16 = 2, UDE_DT_BF16 = 3 };
+enum { UDE_GATE_IDENTITY = 0, UDE_GATE_TANH = 1, UDE_GATE_RBF = 2 /* exp(-x^2) */, UDE_GATE_RELU = 3, UDE_GATE_SIGMOID = 4,
+       UDE_GATE_SWISH = 5 /* x sigmoid(x) */, UDE_GATE_GELU_TANH = 6, UDE_GATE_GELU_ERF = 7 };
+/* y = (act(Wg x) .* (Wu x)) -> Wd, column by column:  y_j = Wd (act(Wg x_j) .* (Wu x_j)),  x: D x T, Wg, Wu: F x D, Wd: O x F, y: O x T
+ * column-major (column j = sample / token j).  Products are summed in Float32 and act is evaluated in Float32 for every dtype; act(..) .*
+ * (..) and, in the pullback, the two cotangents of the hidden layer are rounded to dtype where they enter the next product. */
+typedef struct {
+    int32_t dtype;    /* UDE_DT_F32 / F16 / BF16: x, weights, y, cotangents, gradients */
+    int32_t act;      /* UDE_GATE_* */
+    int32_t w_order;  /* 0: weights out x in column-major (vec(W), consecutive outputs adjacent: Flux / Lux); 1: consecutive INPUTS of one output adjacent */
+    int32_t reserved; /* 0 */
+    int64_t T, D, F, O; /* columns (0 is allowed), inputs, hidden width, outputs; each < 2^31 */
+    int64_t ldx, ldy;   /* elements between the columns of x; of y (forward) or dy (pullback) */
+    int64_t ldg, ldu, ldd; /* elements between the columns (w_order 0) or rows (w_order 1) of Wg, Wu, Wd */
+} ude_gated_ffn_desc;
+/* *bytes = workspace (256-byte aligned) of a forward (pullback = 0) or pullback (1) call */
+int ude_gated_ffn_workspace(const ude_gated_ffn_desc* d, int32_t pullback, int64_t* bytes);
+/* gate, up (F x T floats each, leading dimension F; both or neither NULL) receive Wg x and Wu x for the pullback.  No output may overlap
+ * an input, the workspace or another output. */
+int ude_gated_ffn_forward_dev(ude_ctx* ctx, const ude_gated_ffn_desc* d, const void* x, const void* wg, const void* wu, const void* wd,
+                              void* y, float* gate, float* up, void* ws, int64_t ws_bytes);
+/* cotangent dy (O x T) -> dx (D x T), dwg, dwu, dwd in the order of the weights, all without gaps (each may be NULL: not computed) */
+int ude_gated_ffn_backward_dev(ude_ctx* ctx, const ude_gated_ffn_desc* d, const void* x, const void* wg, const void* wu, const void* wd,
+                               const float* gate, const float* up, const void* dy, void* dx, void* dwg, void* dwu, void* dwd,
+                               void* ws, int64_t ws_bytes);
+
+/* One tensor of an AdamW step: n elements, any alignment of the element type.  Moments: state_bits 32: m, v are floats (doubles for
+ * UDE_DT_F64); state_bits 8: m int8 codes, v uint8 codes, one float of m_scale and of v_scale per UDE_ADAMW_BLOCK consecutive elements
+ * (the last block of a tensor may be short): m = a sign(q) (q/127)^2, v = c (r/255)^4 with a = max |m|, c = max v of the block,
+ * q = sign(m) round(127 sqrt(|m|/a)), r = round(255 (v/c)^(1/4)) and r >= 1 where v > 0 (no zero denominator out of a positive v).  Codes
+ * are decided in Float64.  All zeros is the start of every state.  master: n floats holding the parameters of a 16-bit tensor to 32 bits (updated; the
+ * parameters are then its rounding), or NULL. */
+#define UDE_ADAMW_BLOCK 256
+typedef struct {
+    void* param;
+    const void* grad;
+    float* master;
+    void* m;
+    void* v;
+    float* m_scale;
+    float* v_scale;
+    int64_t n;
+    double weight_decay;
+} ude_adamw_tensor;
+/* m <- b1 m + (1 - b1) s g;  v <- b2 v + (1 - b2) (s g)^2;  p <- p (1 - eta wd) - eta (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)
+ * with s = clip[1] (1 without clip).  t = step, or *step_dev where that is given (read when the call runs: the caller counts, also in a
+ * captured graph); t >= 1. */
+typedef struct {
+    int32_t param_dtype, grad_dtype; /* equal, or grad UDE_DT_F32 with a 16-bit param; all tensors of a call alike */
+    int32_t state_bits;              /* 32 or 8 (Float64 parameters: 32, the moments are then doubles) */
+    int32_t skip_nonfinite;          /* 1: leave everything as it was where clip[0] is not finite */
+    int64_t step;
+    double eta, beta1, beta2, eps;
+    const int64_t* step_dev;         /* device, or NULL */
+    const double* clip;              /* device: {norm, factor} as ude_grad_norm_dev leaves them, or NULL */
+} ude_adamw_opts;
+int ude_adamw_step_dev(ude_ctx* ctx, const ude_adamw_opts* o, int64_t ntensors, const ude_adamw_tensor* tensors /* host array */);
+/* the values that 8-bit moments stand for: m_out[i], v_out[i] = floats of tensors[i] (param, grad, master are not read) */
+int ude_adamw_moments_dev(ude_ctx* ctx, int64_t ntensors, const ude_adamw_tensor* tensors, float* const* m_out, float* const* v_out);
+/* out (device) = {norm, factor}: norm = sqrt of the sum of squares of all elements of all tensors, factor = min(1, max_norm / norm)
+ * (1 where norm is 0 or max_norm is not positive; NaN where norm is NaN).  Summed in Float64 in a fixed order: the same bits every time.
+ * grads, n: host arrays. */
+int ude_grad_norm_workspace(int64_t ntensors, const int64_t* n, int64_t* bytes);
+int ude_grad_norm_dev(ude_ctx* ctx, int32_t dtype, int64_t ntensors, const void* const* grads, const int64_t* n, double max_norm,
+                      double* out, void* ws, int64_t ws_bytes);
+
 /* debugging aid for parity work: record (t, dt, EEst, q, accepted) of every step attempt of trajectory
  * `traj` (forward rows [0,cap), backward rows [cap,2cap), 5 doubles each); traj < 0 switches it off */
 int ude_set_trace(ude_ctx* ctx, int64_t traj, int32_t cap);

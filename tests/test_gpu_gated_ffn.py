@@ -1,0 +1,211 @@
+"""The gated feed-forward block against its Float64 statement, entry by entry within the rounding bounds of tests/_training_ops.py."""
+import ctypes as C
+
+import pytest
+
+torch = pytest.importorskip("torch")
+import _training_ops as R  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+KINDS = [torch.bfloat16, torch.float16, torch.float32]
+IDS = ["bf16", "fp16", "fp32"]
+# (T, D, F, O): single elements, odd sizes, exact tiles, one over a tile, rows that are and are not 16-byte aligned, few and many samples
+SIZES = [(1, 1, 1, 1), (1, 64, 64, 64), (2, 300, 500, 128), (3, 5, 7, 9), (16, 512, 200, 96), (17, 100, 110, 100), (33, 1000, 72, 40),
+         (64, 64, 64, 64), (65, 96, 130, 33), (130, 257, 66, 129), (300, 128, 64, 256), (513, 136, 264, 520), (1500, 40, 48, 24)]
+
+
+def made(T, D, F, O, kind, rows, seed=0, gap=0):
+    """x, wg, wu, wd, dy on the GPU; gap > 0: every matrix is a view whose gaps hold NaN"""
+    gen = torch.Generator().manual_seed(seed)
+
+    def matrix(r, c, by, by_rows=True):
+        if not by_rows:
+            return matrix(c, r, by).T
+        t = torch.full((r, c + gap), float("nan"), dtype=kind, device="cuda")
+        t[:, :c] = (torch.randn((r, c), generator=gen) * by).to(kind).cuda()
+        return t[:, :c]
+
+    return (matrix(T, D, 1.0), matrix(F, D, D ** -0.5, rows), matrix(F, D, D ** -0.5, rows), matrix(O, F, F ** -0.5, rows), matrix(T, O, 1.0))
+
+
+def check(x, wg, wu, wd, dy, act="swish"):
+    import universal_differential_equations_amd as U
+    want = R.gated(x, wg, wu, wd, act, dy)
+    plain = U.gated_ffn(x, wg, wu, wd, act=act)
+    y, saved = U.gated_ffn(x, wg, wu, wd, act=act, save=True)
+    got = dict(zip(("dx", "dwg", "dwu", "dwd"), U.gated_ffn_pullback(saved, dy)), y=y, gate=saved.gate[0], up=saved.gate[1])
+    for name, value in got.items():
+        assert value.shape == want[name][0].shape and (name in ("gate", "up") or value.dtype == x.dtype)
+        assert R.within(value, want[name]) <= 1, (name, R.within(value, want[name]))
+    assert R.within(plain, want["y"]) <= 1
+    for name, w in zip(("dwg", "dwu", "dwd"), (wg, wu, wd)):
+        if min(w.shape) > 1:
+            assert (got[name].stride(1) == 1) == (w.stride(1) == 1)
+    return got
+
+
+@pytest.mark.parametrize("rows", [True, False], ids=["rows", "cols"])
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_forward_and_pullback(size, kind, rows):
+    check(*made(*size, kind, rows))
+
+
+@pytest.mark.parametrize("act", sorted(R.ACTS))
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+def test_activations(act, kind):
+    check(*made(70, 64, 100, 40, kind, True, seed=1), act=act)
+
+
+@pytest.mark.parametrize("rows", [True, False], ids=["rows", "cols"])
+@pytest.mark.parametrize("gap", [1, 8, 24])
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+def test_views_with_gaps(kind, gap, rows):
+    """leading dimensions larger than the rows, NaN in the gaps: nothing outside the matrices is used"""
+    check(*made(37, 72, 88, 56, kind, rows, seed=2, gap=gap))
+    check(*made(140, 264, 136, 72, kind, rows, seed=3, gap=gap))
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+def test_views_that_start_off_alignment(kind):
+    """one element behind an aligned address; gate and up weights as halves of one matrix; x with more than two axes"""
+    x, wg, wu, wd, dy = made(40, 65, 80, 33, kind, True, seed=4)
+    check(x[:, 1:], wg[:, 1:], wu[:, 1:], wd, dy)
+    both = torch.cat((wg, wu))
+    check(x, both[:80], both[80:], wd, dy)
+    import universal_differential_equations_amd as U
+    y, saved = U.gated_ffn(x.view(5, 8, 65), wg, wu, wd, save=True)
+    dx = U.gated_ffn_pullback(saved, dy.view(5, 8, 33))[0]
+    flat, saved2 = U.gated_ffn(x, wg, wu, wd, save=True)
+    assert y.shape == (5, 8, 33) and dx.shape == (5, 8, 65)
+    assert torch.equal(y.view(40, 33), flat) and torch.equal(dx.view(40, 65), U.gated_ffn_pullback(saved2, dy)[0])
+
+
+@pytest.mark.parametrize("size", [(1, 2048, 1100, 640), (7, 640, 2048, 1100), (300, 1100, 640, 2048), (1030, 512, 776, 512), (2100, 64, 520, 72), (4000, 200, 72, 136)],
+                         ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+def test_larger(size, kind):
+    for rows in (True, False):
+        check(*made(*size, kind, rows, seed=5))
+
+
+def test_against_differences():
+    """directional derivatives of sum(y * c) by central differences of the Float64 statement"""
+    import universal_differential_equations_amd as U
+    T, D, F, O = 9, 20, 30, 12
+    x, wg, wu, wd, c = made(T, D, F, O, torch.float32, True, seed=6)
+    _, saved = U.gated_ffn(x, wg, wu, wd, act="gelu_tanh", save=True)
+    grads = U.gated_ffn_pullback(saved, c)
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    args = [t.double() for t in (x, wg, wu, wd)]
+
+    def loss(*a):
+        return float((R.ACTS["gelu_tanh"][0](a[0] @ a[1].T) * (a[0] @ a[2].T) @ a[3].T * c.double()).sum())
+
+    for i, g in enumerate(grads):
+        d = torch.randn(args[i].shape, generator=gen, device="cuda", dtype=torch.float64)
+        at = [[a + (s * 1e-5 * d if j == i else 0) for j, a in enumerate(args)] for s in (1, -1)]
+        slope = (loss(*at[0]) - loss(*at[1])) / 2e-5
+        # truncation (1e-5)^2 and Float64 rounding / 1e-5 are below 1e-8 of the terms; Float32 sums of up to 30 terms: 1e-5
+        assert abs(slope - float((g.double() * d).sum())) <= 1e-5 * float((g.double() * d).abs().sum())
+
+
+def test_rows_are_independent_and_non_finite_rows_stay_alone():
+    import universal_differential_equations_amd as U
+    x, wg, wu, wd, _ = made(70, 96, 64, 48, torch.bfloat16, True, seed=8)
+    y = U.gated_ffn(x, wg, wu, wd)
+    bad = x.clone()
+    bad[3, 5], bad[69, 0] = float("nan"), float("inf")
+    z = U.gated_ffn(bad, wg, wu, wd)
+    keep = [i for i in range(70) if i not in (3, 69)]
+    assert torch.equal(z[keep], y[keep]) and not torch.isfinite(z[3]).any() and not torch.isfinite(z[69]).all()
+
+
+def test_no_samples_and_partial_pullbacks():
+    import universal_differential_equations_amd as U
+    x, wg, wu, wd, dy = made(0, 24, 16, 40, torch.float16, False)
+    y, saved = U.gated_ffn(x, wg, wu, wd, save=True)
+    dx, dwg, dwu, dwd = U.gated_ffn_pullback(saved, dy)
+    assert y.shape == (0, 40) and dx.shape == (0, 24)
+    assert not dwg.any() and not dwu.any() and not dwd.any() and dwg.shape == (16, 24) and dwd.shape == (40, 16)
+    x, wg, wu, wd, dy = made(21, 24, 16, 40, torch.float16, False)
+    _, saved = U.gated_ffn(x, wg, wu, wd, save=True)
+    every = U.gated_ffn_pullback(saved, dy)
+    for names in (("x",), ("w_up",), ("w_gate", "w_down"), ()):
+        some = U.gated_ffn_pullback(saved, dy, need=names)  # (and a second, third, ... pullback of one forward)
+        for name, a, b in zip(("x", "w_gate", "w_up", "w_down"), some, every):
+            assert (a is None) == (name not in names) and (a is None or torch.equal(a, b))
+
+
+def test_output_rows_with_gaps_are_left_alone():
+    """ldy > O through the C entry: what lies between the rows of y, and behind its last row, keeps its bits"""
+    from universal_differential_equations_amd import _lib
+    from universal_differential_equations_amd.layers import _Block
+    for T, D, F, O in ((5, 40, 24, 20), (70, 72, 136, 90)):
+        x, wg, wu, wd, _ = made(T, D, F, O, torch.bfloat16, True, seed=9)
+        b = _Block(x, wg, wu, wd, "swish")
+        b.D.ldy = O + 6
+        y = torch.full((T + 1, O + 6), 7.0, dtype=torch.bfloat16, device="cuda")
+        ws = b.workspace(0)
+        b.bind()
+        b.eng.check(b.eng.L.ude_gated_ffn_forward_dev(b.eng.h, C.byref(b.D), *(t.data_ptr() for t in (x, wg, wu, wd, y)), None, None, ws.data_ptr(), ws.numel()))
+        assert bool((y[:, O:] == 7).all()) and bool((y[T] == 7).all())
+        assert R.within(y[:T, :O], R.gated(x, wg, wu, wd, "swish")["y"]) <= 1
+        assert _lib.GATE["swish"] == b.D.act
+
+
+def test_streams_and_graphs():
+    """the same bits on a side stream, and from two captured graphs that are replayed in turn with other inputs and eager work between"""
+    import universal_differential_equations_amd as U
+    sets = [made(150, 136, 200, 72, torch.bfloat16, True, seed=s) for s in (10, 11)]
+
+    def work(s):
+        y, saved = U.gated_ffn(*s[:4], save=True)
+        return (y,) + U.gated_ffn_pullback(saved, s[4])
+
+    want = [work(s) for s in sets]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = work(sets[0])
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
+    torch.cuda.synchronize()
+    held = [[t.clone() for t in s] for s in sets]
+    graphs, outs = [], []
+    for s in held:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(work(s))
+        graphs.append(g)
+    for turn in range(3):
+        for i in (0, 1):
+            src = sets[(i + turn) % 2]
+            for a, b in zip(held[i], src):
+                a.copy_(b)
+            graphs[i].replay()
+        eager = work(sets[turn % 2])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(eager, want[turn % 2]))
+        for i in (0, 1):
+            assert all(torch.equal(a, b) for a, b in zip(outs[i], want[(i + turn) % 2])), (turn, i)
+
+
+def test_two_threads():
+    import threading
+    import universal_differential_equations_amd as U
+    sets = [made(90, 72, 104, 40, torch.float32, False, seed=s) for s in (12, 13)]
+    want = [U.gated_ffn(*s[:4]) for s in sets]
+    torch.cuda.synchronize()
+    bad = []
+
+    def go(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                if not torch.equal(U.gated_ffn(*sets[i][:4]), want[i]):
+                    bad.append(i)
+
+    ts = [threading.Thread(target=go, args=(i,)) for i in (0, 1)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert not bad

@@ -57,6 +57,31 @@ class HjbDesc(C.Structure):
                 ("beta1", C.c_double), ("beta2", C.c_double), ("dtmax", C.c_double)]
 
 
+DTYPE_CODE = {"float64": 0, "float32": 1, "float16": 2, "bfloat16": 3}   # UDE_DT_*
+GATE = dict(ACT, sigmoid=4, swish=5, gelu_tanh=6, gelu_erf=7)            # UDE_GATE_*
+ADAMW_BLOCK = 256
+
+
+class GatedFfnDesc(C.Structure):
+    """ude_gated_ffn_desc"""
+    _fields_ = [("dtype", C.c_int32), ("act", C.c_int32), ("w_order", C.c_int32), ("reserved", C.c_int32),
+                ("T", C.c_int64), ("D", C.c_int64), ("F", C.c_int64), ("O", C.c_int64), ("ldx", C.c_int64), ("ldy", C.c_int64),
+                ("ldg", C.c_int64), ("ldu", C.c_int64), ("ldd", C.c_int64)]
+
+
+class AdamwTensor(C.Structure):
+    """ude_adamw_tensor"""
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("master", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p),
+                ("m_scale", C.c_void_p), ("v_scale", C.c_void_p), ("n", C.c_int64), ("weight_decay", C.c_double)]
+
+
+class AdamwOpts(C.Structure):
+    """ude_adamw_opts"""
+    _fields_ = [("param_dtype", C.c_int32), ("grad_dtype", C.c_int32), ("state_bits", C.c_int32), ("skip_nonfinite", C.c_int32),
+                ("step", C.c_int64), ("eta", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+                ("step_dev", C.c_void_p), ("clip", C.c_void_p)]
+
+
 class UdeError(RuntimeError):
     def __init__(self, code, msg):
         super().__init__("udecore error %d: %s" % (code, msg))
@@ -73,7 +98,9 @@ EXPORTS = ["ude_version", "ude_create", "ude_destroy", "ude_last_error", "ude_se
            "ude_hjb_net", "ude_hjb_last_kernel_ms", "ude_hjb_debug_read", "ude_hjb_last_failures",
            "ude_comm_unique_id", "ude_comm_create", "ude_comm_create_local", "ude_comm_destroy", "ude_allreduce_grad",
            "ude_allreduce_grad_local", "ude_allreduce_grad_p2p", "ude_comm_create_p2p", "ude_comm_p2p_connect",
-           "ude_allreduce_grad_p2p_mp", "ude_comm_p2p_status", "ude_comm_p2p_disconnect", "ude_pack_counters_dev"]
+           "ude_allreduce_grad_p2p_mp", "ude_comm_p2p_status", "ude_comm_p2p_disconnect", "ude_pack_counters_dev",
+           "ude_gated_ffn_workspace", "ude_gated_ffn_forward_dev", "ude_gated_ffn_backward_dev", "ude_adamw_step_dev",
+           "ude_adamw_moments_dev", "ude_grad_norm_workspace", "ude_grad_norm_dev"]
 
 
 def load():
@@ -137,6 +164,13 @@ def load():
     L.ude_comm_p2p_status.argtypes = [vp, C.POINTER(i32)]
     L.ude_comm_p2p_disconnect.argtypes = [vp]
     L.ude_pack_counters_dev.argtypes = [vp, i64, vp, vp, i32]
+    L.ude_gated_ffn_workspace.argtypes = [C.POINTER(GatedFfnDesc), i32, C.POINTER(i64)]
+    L.ude_gated_ffn_forward_dev.argtypes = [vp, C.POINTER(GatedFfnDesc)] + [vp] * 8 + [i64]
+    L.ude_gated_ffn_backward_dev.argtypes = [vp, C.POINTER(GatedFfnDesc)] + [vp] * 12 + [i64]
+    L.ude_adamw_step_dev.argtypes = [vp, C.POINTER(AdamwOpts), i64, vp]
+    L.ude_adamw_moments_dev.argtypes = [vp, i64, vp, vp, vp]
+    L.ude_grad_norm_workspace.argtypes = [i64, vp, C.POINTER(i64)]
+    L.ude_grad_norm_dev.argtypes = [vp, i32, i64, vp, vp, C.c_double, vp, vp, i64]
     L.ude_hjb_debug_read.argtypes = [vp, i32, i64, i64, vp]
     L.ude_hjb_last_kernel_ms.argtypes = [vp, C.POINTER(C.c_float), C.POINTER(C.c_float)]
     L.ude_set_trace.argtypes = [vp, i64, i32]

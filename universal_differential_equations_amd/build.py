@@ -26,6 +26,9 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # (HIP's __fsqrt_rn intrinsic is the NATIVE approximate sqrt unless OCML_BASIC_ROUNDED_OPERATIONS is defined: not used)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fhip-fp32-correctly-rounded-divide-sqrt"]
 
+# packed Float32 instructions (v_pk_fma_f32 and the like) are kept out of the units that would be full of them
+NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 # (model id, C++ model type, lanes per trajectory, kernel variant VAR [, block threads [, algorithms]]).  VAR is a template
 # parameter of adj_kernel (1 = default; 2 = __launch_bounds__ for two waves per SIMD; 9 = lambda-only timing experiment):
 # variants must differ in their template arguments, a macro-only difference gives one mangled name and the linker keeps one body
@@ -340,6 +343,9 @@ def kernel_work(objdir, extra):
     work.append((os.path.join(CSRC, "ude_node_lsf.hip"), os.path.join(objdir, "ude_node_lsf.o"), [] + extra, os.path.join(objdir, "ude_node_lsf.log")))
     # the multi-GPU exchange step (RCCL bound with dlopen, one-shot P2P reducer), SURVEY.md 8(e)
     work.append((os.path.join(CSRC, "ude_comm.hip"), os.path.join(objdir, "ude_comm.o"), [] + extra, os.path.join(objdir, "ude_comm.log")))
+    # the training operators (gated feed-forward block, AdamW, gradient norm): Float32 arithmetic without the packed forms
+    for unit in ("ude_gated", "ude_optim"):
+        work.append((os.path.join(CSRC, unit + ".hip"), os.path.join(objdir, unit + ".o"), NO_PACKED + extra, os.path.join(objdir, unit + ".log")))
     return work
 
 

@@ -16,7 +16,7 @@ import ctypes as C
 
 import numpy as np
 
-from . import _lib
+from . import _lib, training
 from ._lib import HjbDesc, UdeError
 from .sciml import Engine, _ptr
 
@@ -55,6 +55,17 @@ class ADAM:
 
     def __init__(self, eta=0.001, beta=(0.9, 0.999)):
         self.eta, self.beta, self.eps = eta, beta, 1e-8
+
+
+class ADAMW:
+    """Flux.ADAMW(eta, (0.9, 0.999), decay) = Optimiser(ADAM(eta, beta), WeightDecay(decay)): the update of ADAM plus decay * theta, with,
+    where max_norm is given, ClipNorm(max_norm) in front of it.  The step and the norm are single launches over the parameters in HBM
+    (training.AdamW, training.grad_norm)."""
+
+    def __init__(self, eta=0.001, beta=(0.9, 0.999), decay=0.0, max_norm=None):
+        if not eta > 0:
+            raise ValueError("ADAMW: eta = %r" % (eta,))
+        self.eta, self.beta, self.decay, self.max_norm, self.eps = eta, beta, decay, max_norm, 1e-8
 
 
 class NNPDENS:
@@ -181,6 +192,9 @@ def solve(prob, pdealg, theta0, verbose=False, maxiters=300, trajectories=100, a
     m = torch.zeros_like(theta)
     v = torch.zeros_like(theta)
     b1p, b2p = opt.beta
+    fused = None
+    if isinstance(opt, ADAMW):   # (eta wd of the fused step is Flux's decay, which eta does not scale)
+        fused = training.AdamW([theta], eta=opt.eta, beta=opt.beta, eps=opt.eps, weight_decay=opt.decay / opt.eta)
     losses = []
     for it in range(maxiters):
         loss, g = bs.loss_grad(theta, it=it)
@@ -194,6 +208,9 @@ def solve(prob, pdealg, theta0, verbose=False, maxiters=300, trajectories=100, a
             raise UdeError(_lib.UDE_ERR_TRAJECTORY, "a trajectory failed (retcodes %s)" % sorted(set(bs.retcode.tolist())))
         if lval < pabstol:
             break
+        if fused is not None:
+            fused.step([g], clip=None if opt.max_norm is None else training.grad_norm([g], opt.max_norm))
+            continue
         # Flux.ADAM (0.9): mt = b1 mt + (1-b1) g; vt = b2 vt + (1-b2) g^2; theta -= mt/(1-b1^t) / (sqrt(vt/(1-b2^t)) + eps) * eta
         m.mul_(opt.beta[0]).add_(g, alpha=1 - opt.beta[0])
         v.mul_(opt.beta[1]).addcmul_(g, g, value=1 - opt.beta[1])

@@ -11,7 +11,11 @@ gradient and optimiser state in HBM, nothing crosses PCIe inside the loop).  ADA
 scenario_1's stored losses); `bfgs` is a plain inverse-Hessian BFGS with Armijo backtracking (cheaper per iteration, kept for the
 examples that do not compare with an artifact).
 """
+import ctypes as C
+
 import numpy as np
+
+from . import _lib
 
 
 def _xp(x):
@@ -41,6 +45,228 @@ def adam(loss_grad, theta, eta=0.1, beta=(0.9, 0.999), maxiters=200, callback=No
         theta = theta - eta * (m / (1 - b1t)) / (xp.sqrt(v / (1 - b2t)) + eps)
         b1t *= beta[0]
         b2t *= beta[1]
+    return (last if result == "evaluated" and losses else theta), losses
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# The optimiser step on the device, over many tensors at once (ude_adamw_step_dev, ude_grad_norm_dev)
+# ---------------------------------------------------------------------------------------------------------------
+def _device_list(what, tensors):
+    """the common (device, dtype name) of a list of CUDA tensors"""
+    if not tensors:
+        raise ValueError("%s: an empty list of tensors" % what)
+    dev, dt = tensors[0].device, tensors[0].dtype
+    if dev.type != "cuda":
+        raise ValueError("%s: tensor 0 is on %s, CUDA tensors are needed (there is no CPU fallback)" % (what, dev))
+    name = str(dt)[6:]
+    if name not in _lib.DTYPE_CODE:
+        raise ValueError("%s: tensor 0 is %s: float64, float32, float16 and bfloat16 are supported" % (what, dt))
+    for i, t in enumerate(tensors):
+        if t.device != dev or t.dtype != dt:
+            raise ValueError("%s: tensor %d is %s on %s, tensor 0 %s on %s" % (what, i, t.dtype, t.device, dt, dev))
+    return dev, name
+
+
+def _bound_engine(dev):
+    import torch
+    from .sciml import Engine
+    eng = Engine.get(dev.index)
+    eng.set_stream(torch.cuda.current_stream(dev).cuda_stream)
+    return eng
+
+
+def grad_norm(grads, max_norm=0.0):
+    """float64 CUDA tensor [norm, factor] of a list of CUDA tensors of one dtype: norm = sqrt of the sum of all squares (summed in Float64,
+    the same bits every time), factor = min(1, max_norm / norm) -- what `AdamW.step(grads, clip=...)` multiplies the gradients with.
+    Nothing crosses PCIe.  max_norm <= 0: factor 1 (NaN where the norm is)."""
+    import torch
+    grads = [g if g.is_contiguous() else g.contiguous() for g in grads if g is not None]
+    dev, name = _device_list("grad_norm", grads)
+    n = len(grads)
+    ptrs, sizes = (C.c_void_p * n)(*[g.data_ptr() for g in grads]), (C.c_int64 * n)(*[g.numel() for g in grads])
+    eng = _bound_engine(dev)
+    need = C.c_int64(0)
+    eng.check(eng.L.ude_grad_norm_workspace(n, sizes, C.byref(need)))
+    buf = torch.empty(2 + need.value // 8, dtype=torch.float64, device=dev)   # [norm, factor] and the partial sums behind them
+    eng.check(eng.L.ude_grad_norm_dev(eng.h, _lib.DTYPE_CODE[name], n, ptrs, sizes, float(max_norm), buf.data_ptr(), buf.data_ptr() + 16, need.value))
+    return buf[:2]
+
+
+class AdamW:
+    """AdamW over a list of CUDA tensors of one dtype, one launch for dozens of tensors; updates them in place:
+
+        m = b1 m + (1 - b1) s g,  v = b2 v + (1 - b2) (s g)^2,  p = p (1 - eta wd) - eta (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)
+
+    weight_decay: one number, or one per tensor.  bits = 32: Float32 moments (Float64 for float64 parameters); bits = 8: moments as 8-bit
+    codes with two scales per 256 elements (ude_adamw_tensor).  master=True keeps a Float32 copy of 16-bit parameters that the updates
+    accumulate in.  state: one dict per tensor with "m", "v" (codes: int8, uint8, with "m_scale", "v_scale") and "master" -- tensors that
+    are used as they are, e.g. another instance's `state` out of a checkpoint; step: the steps already done.  capturable=True counts
+    the steps on the device, as a step that is captured into a hipGraph needs.  skip_nonfinite=True leaves everything as it was in a step
+    whose clip[0] is not finite (the step is counted).  A non-finite gradient makes the 8-bit moments of its block of 256 NaN."""
+
+    def __init__(self, params, eta=0.001, beta=(0.9, 0.999), eps=1e-8, weight_decay=0.01, bits=32, master=False, state=None, step=0,
+                 skip_nonfinite=False, capturable=False):
+        import torch
+        self.torch = torch
+        self.params = list(params)
+        self.device, self.dtype = _device_list("AdamW", self.params)
+        half = self.dtype in ("float16", "bfloat16")
+        if bits not in (32, 8) or (bits == 8 and self.dtype == "float64"):
+            raise ValueError("AdamW: bits = %r with %s parameters" % (bits, self.dtype))
+        if master and not half:
+            raise ValueError("AdamW: master copies go with 16-bit parameters, these are %s" % self.dtype)
+        for i, p in enumerate(self.params):
+            if not p.is_contiguous():
+                raise ValueError("AdamW: parameter %d is not contiguous (strides %s)" % (i, p.stride()))
+        used = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size(), i) for i, p in enumerate(self.params) if p.numel())
+        for (_, end, i), (start, _, j) in zip(used, used[1:]):
+            if start < end:
+                raise ValueError("AdamW: parameters %d and %d share memory" % (min(i, j), max(i, j)))
+        n = len(self.params)
+        decay = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
+        if len(decay) != n:
+            raise ValueError("AdamW: %d values of weight_decay for %d parameters" % (len(decay), n))
+        self.eta, self.beta, self.eps, self.bits, self.steps = eta, tuple(beta), eps, bits, int(step)
+        self.skip_nonfinite = bool(skip_nonfinite)
+        self.count = torch.full((1,), self.steps, dtype=torch.int64, device=self.device) if capturable else None
+        if state is not None and len(state) != n:
+            raise ValueError("AdamW: state of %d tensors for %d parameters" % (len(state), n))
+        self._state = [self._make_state(i, master, None if state is None else state[i]) for i in range(n)]
+        self._table = (_lib.AdamwTensor * n)()
+        self._live = [0] * n
+        for i, p in enumerate(self.params):
+            s, t = self._state[i], self._table[i]
+            t.master, t.m, t.v = (s[k].data_ptr() if k in s else None for k in ("master", "m", "v"))
+            t.m_scale, t.v_scale = (s[k].data_ptr() if k in s else None for k in ("m_scale", "v_scale"))
+            t.param, t.n, t.weight_decay = p.data_ptr(), p.numel(), decay[i]
+            self._live[i] = p.numel()
+        self._opts = _lib.AdamwOpts(param_dtype=_lib.DTYPE_CODE[self.dtype], state_bits=bits)
+
+    def _make_state(self, i, master, given):
+        torch, p = self.torch, self.params[i]
+        n, blocks = p.numel(), -(-p.numel() // _lib.ADAMW_BLOCK)
+        if self.bits == 8:
+            want = {"m": (torch.int8, n), "v": (torch.uint8, n), "m_scale": (torch.float32, blocks), "v_scale": (torch.float32, blocks)}
+        else:
+            t = torch.float64 if self.dtype == "float64" else torch.float32
+            want = {"m": (t, n), "v": (t, n)}
+        if master:
+            want["master"] = (torch.float32, n)
+        if given is None:
+            made = {k: torch.zeros(size, dtype=t, device=self.device) for k, (t, size) in want.items() if k != "master"}
+            if master:
+                made["master"] = p.detach().reshape(-1).float()
+            return made
+        if set(given) != set(want):
+            raise ValueError("AdamW: state %d has %s, %s are needed" % (i, sorted(given), sorted(want)))
+        for k, (t, size) in want.items():
+            x = given[k]
+            if x.dtype != t or x.numel() != size or x.device != self.device or not x.is_contiguous():
+                raise ValueError("AdamW: state %d, %s: %s of %d elements on %s, contiguous, is needed" % (i, k, t, size, self.device))
+        return dict(given)
+
+    @property
+    def state(self):
+        """one dict of tensors per parameter (the tensors themselves: copy into them to change the state)"""
+        return [dict(s) for s in self._state]
+
+    def step(self, grads, clip=None):
+        """one update with `grads` (a tensor per parameter, of the parameters' dtype or, for 16-bit parameters, float32; None: that
+        parameter and its moments stay as they are); clip: `grad_norm(...)`'s result, whose factor scales the gradients"""
+        torch, table = self.torch, self._table
+        if len(grads) != len(self.params):
+            raise ValueError("AdamW: %d gradients for %d parameters" % (len(grads), len(self.params)))
+        gdt, keep = None, []
+        for i, (p, g) in enumerate(zip(self.params, grads)):
+            t = table[i]
+            if p.data_ptr() != t.param:
+                self._moved(i)
+            if g is None:
+                t.n = 0
+                continue
+            if gdt is None:
+                gdt = g.dtype
+            if g.dtype != gdt or g.device != self.device or g.numel() != self._live[i]:
+                raise ValueError("AdamW: gradient %d is %s of %d elements on %s; %s of %d on %s is needed"
+                                 % (i, g.dtype, g.numel(), g.device, gdt, self._live[i], self.device))
+            if not g.is_contiguous():
+                g = g.contiguous()
+                keep.append(g)
+            t.grad, t.n = g.data_ptr(), self._live[i]
+        o = self._opts
+        o.grad_dtype = o.param_dtype if gdt is None else _lib.DTYPE_CODE.get(str(gdt)[6:], -1)
+        if clip is not None and (clip.dtype != torch.float64 or clip.numel() != 2 or clip.device != self.device or not clip.is_contiguous()):
+            raise ValueError("AdamW: clip is what grad_norm returns: a float64 tensor [norm, factor] on %s" % self.device)
+        o.clip = None if clip is None else clip.data_ptr()
+        o.skip_nonfinite = int(self.skip_nonfinite)
+        o.eta, (o.beta1, o.beta2), o.eps = self.eta, self.beta, self.eps
+        eng = _bound_engine(self.device)
+        if self.count is not None:
+            self.count.add_(1)
+            o.step_dev = self.count.data_ptr()
+        elif torch.cuda.is_current_stream_capturing():
+            raise ValueError("AdamW: a step that is captured into a graph has to count on the device: capturable=True")
+        o.step = self.steps + 1
+        rc = eng.L.ude_adamw_step_dev(eng.h, C.byref(o), len(table), table)
+        if rc and self.count is not None:
+            self.count.sub_(1)
+        eng.check(rc)
+        self.steps += 1
+
+    def _moved(self, i):
+        """parameter i was given other storage"""
+        p = self.params[i]
+        if p.device != self.device or str(p.dtype)[6:] != self.dtype or p.numel() != self._live[i] or not p.is_contiguous():
+            raise ValueError("AdamW: parameter %d was replaced by %s of %d elements on %s" % (i, p.dtype, p.numel(), p.device))
+        self._table[i].param = p.data_ptr()
+
+    def moments(self, out=None):
+        """[(m, v), ...]: the values of the moments, Float32 (Float64 for float64 parameters); out: pairs of tensors to write 8-bit
+        moments' values to"""
+        torch = self.torch
+        if self.bits != 8:
+            return [(s["m"], s["v"]) for s in self._state]
+        n = len(self.params)
+        if out is None:
+            out = [tuple(torch.empty(k, dtype=torch.float32, device=self.device) for _ in range(2)) for k in self._live]
+        if len(out) != n:
+            raise ValueError("AdamW: %d outputs for %d parameters" % (len(out), n))
+        for i, pair in enumerate(out):
+            for x in pair:
+                if x.dtype != torch.float32 or x.numel() != self._live[i] or x.device != self.device or not x.is_contiguous():
+                    raise ValueError("AdamW: output %d: float32 of %d elements on %s, contiguous, is needed" % (i, self._live[i], self.device))
+        ms, vs = ((C.c_void_p * n)(*[pair[k].data_ptr() for pair in out]) for k in range(2))
+        for i, k in enumerate(self._live):
+            self._table[i].n = k
+        eng = _bound_engine(self.device)
+        eng.check(eng.L.ude_adamw_moments_dev(eng.h, n, self._table, ms, vs))
+        return out
+
+
+def adamw(loss_grad, theta, eta=0.001, beta=(0.9, 0.999), decay=0.01, maxiters=200, callback=None, eps=1e-8, max_norm=None, result="updated"):
+    """`adam` with decoupled weight decay (theta <- theta (1 - eta decay) - ...) and, with max_norm, the gradient scaled to that norm where
+    it is larger.  theta: numpy, or a torch tensor; a CUDA tensor is updated by the fused step and stays on the device."""
+    xp = _xp(theta)
+    cuda = xp is not np and theta.is_cuda
+    theta = theta.clone() if xp is not np else np.array(theta, dtype=np.float64)
+    opt = AdamW([theta], eta=eta, beta=beta, eps=eps, weight_decay=decay) if cuda else None
+    m, v = (None, None) if cuda else (xp.zeros_like(theta), xp.zeros_like(theta))
+    losses, last = [], theta
+    for it in range(maxiters):
+        loss, g = loss_grad(theta)
+        losses.append(float(loss))
+        last = theta.clone() if cuda and result == "evaluated" else theta
+        if callback is not None and callback(theta.clone() if cuda else theta, losses[-1]):   # (the fused step updates theta in place)
+            break
+        if cuda:
+            opt.step([g], clip=None if max_norm is None else grad_norm([g], max_norm))
+            continue
+        if max_norm is not None:
+            norm = xp.sqrt((g * g).sum())
+            g = g * (max_norm / norm) if norm > max_norm else g
+        m = beta[0] * m + (1 - beta[0]) * g
+        v = beta[1] * v + (1 - beta[1]) * g * g
+        theta = theta * (1 - eta * decay) - eta * (m / (1 - beta[0] ** (it + 1))) / (xp.sqrt(v / (1 - beta[1] ** (it + 1))) + eps)
     return (last if result == "evaluated" and losses else theta), losses
 
 
