@@ -89,6 +89,15 @@ def test_larger(size, kind):
         check(*made(*size, kind, rows, seed=5))
 
 
+@pytest.mark.parametrize("size", [(72, 2052, 4100, 264), (2100, 328, 2310, 2050), (4100, 2052, 136, 72), (4100, 72, 2056, 136), (4096, 256, 2048, 2048)],
+                         ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("kind", KINDS[:2], ids=IDS[:2])
+def test_many_large_tiles(size, kind):
+    """enough output for the largest tiles in each of the products, inner sizes that end inside a step of 64 among them"""
+    for rows in (True, False):
+        check(*made(*size, kind, rows, seed=15))
+
+
 def test_against_differences():
     """directional derivatives of sum(y * c) by central differences of the Float64 statement"""
     import universal_differential_equations_amd as U

@@ -97,7 +97,8 @@ struct Args {
     int M, N, K;
     int nseg;      // EPI_STORE: products summed into one output, C[0] = sum_s A[s] B[s]^T
     int act;
-    int vecA, vecB;  // 16-byte loads allowed: base and leading dimension aligned
+    int vecA, vecB;  // 16-byte loads allowed: base and leading dimension aligned (gemm_any)
+    int vecC;        // stores of four consecutive columns allowed
     float *gate, *up;        // EPI_GATE: stored if not NULL; EPI_PULL: read; leading dimension N
     void *dg, *du, *h;       // EPI_PULL: dg and du with leading dimension ldc[0], h with ldc[1]
 };
@@ -116,6 +117,71 @@ static __device__ inline void load8(const E* p, int64_t left, bool row, int vec,
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i] = (row && i < left) ? p[i] : (E)0;
+    }
+}
+
+// What a tile kernel does with the four consecutive columns n.. of row m that a lane holds (v = Wu's product for EPI_GATE)
+template <class T, int EPI>
+static __device__ inline void finish(const Args& a, int z, int m, int n, f4 c, f4 v) {
+    typedef typename T::E E;
+    typedef E E4 __attribute__((ext_vector_type(4)));
+    if (n >= a.N) return;
+    const int64_t at = (int64_t)m * a.N + n;
+    if constexpr (EPI == EPI_STORE) {
+        E* to = (E*)a.C[z] + (int64_t)m * a.ldc[z] + n;
+        const E4 o = {T::from(c[0]), T::from(c[1]), T::from(c[2]), T::from(c[3])};
+        if (a.vecC && n + 4 <= a.N)
+            *(E4*)to = o;
+        else
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (n + q < a.N) to[q] = o[q];
+    } else if constexpr (EPI == EPI_GATE) {
+        E* to = (E*)a.C[0] + (int64_t)m * a.ldc[0] + n;
+        E4 o;
+        float slope;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o[q] = T::from(gate_act(a.act, c[q], &slope) * v[q]);
+        if (a.vecC && n + 4 <= a.N) {
+            *(E4*)to = o;
+            if (a.gate) {
+                *(f4*)(a.gate + at) = c;
+                *(f4*)(a.up + at) = v;
+            }
+        } else
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (n + q < a.N) {
+                    to[q] = o[q];
+                    if (a.gate) a.gate[at + q] = c[q], a.up[at + q] = v[q];
+                }
+    } else {
+        const bool four = a.vecC && n + 4 <= a.N;
+        f4 gv = {}, uv = {};
+        if (four)
+            gv = *(const f4*)(a.gate + at), uv = *(const f4*)(a.up + at);
+        else
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (n + q < a.N) gv[q] = a.gate[at + q], uv[q] = a.up[at + q];
+        E4 og, ou, oh;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float slope;
+            const float av = gate_act(a.act, gv[q], &slope);
+            og[q] = T::from(c[q] * uv[q] * slope);
+            ou[q] = T::from(c[q] * av);
+            oh[q] = T::from(av * uv[q]);
+        }
+        const int64_t to = (int64_t)m * a.ldc[0] + n, th = (int64_t)m * a.ldc[1] + n;
+        if (four) {
+            *(E4*)((E*)a.dg + to) = og;
+            *(E4*)((E*)a.du + to) = ou;
+            *(E4*)((E*)a.h + th) = oh;
+        } else
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (n + q < a.N) ((E*)a.dg)[to + q] = og[q], ((E*)a.du)[to + q] = ou[q], ((E*)a.h)[th + q] = oh[q];
     }
 }
 
@@ -188,41 +254,209 @@ __global__ __launch_bounds__(256) void gemm_any(const Args a) {
     for (int i = 0; i < 2; ++i) {
         const int m = m0 + wm * 32 + i * 16 + r;
         if (m >= a.M) continue;
-        if constexpr (EPI == EPI_GATE) {
+        if constexpr (EPI == EPI_GATE)
+            finish<T, EPI>(a, 0, m, n0 + wn * 16 + g * 4, acc[i][0], acc[i][1]);
+        else
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int n = n0 + wn * 16 + g * 4 + q;
-                if (n >= a.N) continue;
-                float slope;
-                const float gv = acc[i][0][q], uv = acc[i][1][q];
-                ((E*)a.C[0])[(int64_t)m * a.ldc[0] + n] = T::from(gate_act(a.act, gv, &slope) * uv);
-                if (a.gate) {
-                    a.gate[(int64_t)m * a.N + n] = gv;
-                    a.up[(int64_t)m * a.N + n] = uv;
-                }
+            for (int j = 0; j < 2; ++j) finish<T, EPI>(a, z, m, n0 + wn * 32 + j * 16 + g * 4, acc[i][j], f4{});
+    }
+}
+
+// ---- the tile kernel of the 16-bit kinds ------------------------------------------------------------------------------------------
+// A BM x BN tile of C by NWM x NWN wavefronts; K in steps of 64 through two LDS buffers that buffer_load .. lds fills 16 bytes a lane,
+// straight from memory: while step k is multiplied, step k + 1 is on its way.  What a descriptor's record count does not cover is
+// filled with zeros, so that edges cost no branches; a lane outside asks for OUTSIDE.
+//
+// LDS layouts (a 1 KB piece is one instruction of one wavefront, lane l at 16 l):
+//   "K" operand [row][64 k], 128 B a row: the 16-byte chunk c of row r lies at chunk c ^ (r & 7) -- 16 lanes that read chunk c of 16
+//       consecutive rows touch every bank once.
+//   "R" operand [64 k][W rows] (W = 128 or 64): read through ds_read_b64_tr_b16, which hands each lane four consecutive k of one row; the
+//       32-byte pair P of k-row k lies at P ^ spread(k), which spreads the 8 k-rows that are read together over the banks.
+constexpr unsigned OUTSIDE = 0x80000000u;
+typedef int i4 __attribute__((ext_vector_type(4)));
+
+static __device__ inline i4 records(const char* base, int64_t bytes) {
+    const uint64_t p = (uint64_t)base;
+    const int64_t n = bytes < 0 ? 0 : bytes > 0x7ffffffc ? 0x7ffffffc : (bytes + 3) & ~(int64_t)3;
+    i4 r;
+    r[0] = __builtin_amdgcn_readfirstlane((int)p);
+    r[1] = __builtin_amdgcn_readfirstlane((int)(p >> 32) & 0xffff);
+    r[2] = __builtin_amdgcn_readfirstlane((int)n);
+    r[3] = 0x00020000;
+    return r;
+}
+static __device__ inline void to_lds(unsigned at, unsigned off, i4 r) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(r) : "m0");
+}
+static __device__ inline unsigned lds_address(const void* p) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p; }
+
+template <int W>
+static __device__ constexpr int spread(int k) {
+    return W == 128 ? (k & 3) | ((k >> 3) & 1) << 2 : ((k >> 1) & 1) | ((k >> 3) & 1) << 1;
+}
+
+// One operand of a tile: ROWS rows (of HALVES matrices, ROWS / HALVES each) by 64 k
+template <class T, bool KC, int ROWS, int NW, int HALVES>
+struct Operand {
+    typedef typename T::E E;
+    static constexpr int N = ROWS / 8 / NW;                            // 1 KB pieces of a wavefront
+    static constexpr int W = KC ? 0 : (ROWS / HALVES >= 128 ? 128 : 64);  // width of a sub-tile of an "R" operand
+    static constexpr int BYTES = ROWS * 128;
+    static_assert(N * 8 * NW == ROWS && N % HALVES == 0, "pieces");
+    const char* base[HALVES];
+    int64_t left[HALVES], step[HALVES];
+    unsigned off[N];
+    int koff;  // "K": first k of this lane's chunks; "R": not used
+
+    // rows row0.. of matrices with `rows` rows and K columns
+    __device__ inline void init(const void* const* p, const int64_t* ld, int row0, int rows, int K, int wave, int lane) {
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+            if constexpr (KC) {
+                base[h] = (const char*)p[h] + (int64_t)row0 * ld[h] * 2;
+                left[h] = ((int64_t)(rows - 1 - row0) * ld[h] + K) * 2;
+                step[h] = 128;
+            } else {
+                base[h] = (const char*)p[h] + (int64_t)row0 * 2;
+                left[h] = ((int64_t)(K - 1) * ld[h] + rows - row0) * 2;
+                step[h] = 128 * ld[h];
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int n = n0 + wn * 32 + j * 16 + g * 4 + q;
-                    if (n >= a.N) continue;
-                    const float c = acc[i][j][q];
-                    if constexpr (EPI == EPI_STORE) {
-                        ((E*)a.C[z])[(int64_t)m * a.ldc[z] + n] = T::from(c);
-                    } else {
-                        const int64_t at = (int64_t)m * a.N + n;
-                        const float gv = a.gate[at], uv = a.up[at];
-                        float slope;
-                        const float av = gate_act(a.act, gv, &slope);
-                        const int64_t to = (int64_t)m * a.ldc[0] + n;
-                        ((E*)a.dg)[to] = T::from(c * uv * slope);
-                        ((E*)a.du)[to] = T::from(c * av);
-                        ((E*)a.h)[(int64_t)m * a.ldc[1] + n] = T::from(av * uv);
-                    }
-                }
         }
+        koff = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int h = i / (N / HALVES), piece = (i % (N / HALVES)) * NW + wave;
+            if constexpr (KC) {
+                const int r = piece * 8 + (lane >> 3);
+                koff = ((lane & 7) ^ (lane >> 3)) * 8;
+                off[i] = row0 + r < rows ? (unsigned)(r * (int)ld[h] * 2 + koff * 2) : OUTSIDE;
+            } else {
+                constexpr int PP = W / 8, RP = 512 / W;  // pieces of a sub-tile; k-rows of a piece
+                const int sub = piece / PP, k = (piece % PP) * RP + lane / (W / 8), u = lane % (W / 8);
+                const int r = sub * W + ((u >> 1) ^ spread<W>(k)) * 16 + (u & 1) * 8;
+                off[i] = row0 + r < rows ? (unsigned)(k * (int)ld[h] * 2 + r * 2) : OUTSIDE;
+            }
+        }
+    }
+    // issues the loads of one step to LDS at `at`, then moves on; kleft = columns from this step on
+    __device__ inline void load(unsigned at, int wave, int lane, int kleft, E* lds) {
+        i4 r[HALVES];
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) r[h] = records(base[h], left[h]);
+        const bool full = !KC || kleft >= 64;
+        if (full || kleft % 8 == 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const unsigned o = full || koff < kleft ? off[i] : OUTSIDE;
+                to_lds(at + (i * NW + wave) * 1024, o, r[i / (N / HALVES)]);
+            }
+        } else {  // the last step of a K that 8 does not divide: element by element
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                s8 v = {};
+                if (off[i] != OUTSIDE) {
+                    const E* p = (const E*)(base[i / (N / HALVES)] + off[i]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (koff + e < kleft) v[e] = p[e];
+                }
+                *(s8*)((char*)lds + (i * NW + wave) * 1024 + lane * 16) = v;
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) base[h] += step[h], left[h] -= step[h];
+    }
+    // the 8 k of row `row` (a multiple of 16, plus lane & 15) that a lane feeds to the matrix instruction of k-half kk
+    static __device__ inline s8 fragment(const char* lds, int row, int kk, int lane) {
+        const int g = lane >> 4;
+        if constexpr (KC) {
+            return *(const s8*)(lds + (row + (lane & 15)) * 128 + (((kk * 4 + g) ^ (lane & 7)) << 4));
+        } else {
+            const int kr = g * 8 + ((lane & 15) >> 2);
+            const char* p = lds + (row / W) * (W * 128) + kr * (W * 2) + ((((row % W) >> 4) ^ spread<W>(kr)) << 5) + (lane & 3) * 8 + kk * 32 * (W * 2);
+            typedef __attribute__((address_space(3))) s4* P;
+            const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)p), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(p + 4 * (W * 2)));
+            return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+};
+
+template <class T, int EPI, bool AK, bool BKc, int BM, int BN, int NWM, int NWN>
+__global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_tile(const Args a) {
+    constexpr int NW = NWM * NWN, FM = BM / NWM / 16, FN = BN / NWN / 16, HALVES = EPI == EPI_GATE ? 2 : 1;
+    constexpr int NT = BN / HALVES;  // output columns of a tile
+    typedef Operand<T, AK, BM, NW, 1> OA;
+    typedef Operand<T, BKc, BN, NW, HALVES> OB;
+    constexpr int STAGE = OA::BYTES + OB::BYTES;
+    __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % NWM, wn = wave / NWM;
+    const int z = blockIdx.z;
+    // workgroup b runs on XCD b % 8: each XCD takes a contiguous run of tiles, in groups of 8 rows of tiles, so that its L2 holds the
+    // rows of A of a group and a few columns of B
+    const int nm = (a.M + BM - 1) / BM, nn = (a.N + NT - 1) / NT, tiles = nm * nn;
+    int t = (int)blockIdx.x;
+    {
+        const int q = tiles / 8, r = tiles % 8, x = t % 8, l = t / 8;
+        t = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + l;
+    }
+    constexpr int GM = 8;
+    const int group = t / (GM * nn), gm0 = group * GM, gsize = nm - gm0 < GM ? nm - gm0 : GM;
+    const int m0 = (gm0 + (t - group * GM * nn) % gsize) * BM, n0 = (t - group * GM * nn) / gsize * NT;
+
+    f4 acc[FM][FN] = {};
+    OA oa;
+    OB ob;
+    const unsigned at = __builtin_amdgcn_readfirstlane(lds_address(lds));
+    const int per = (a.K + 63) / 64, steps = per * a.nseg;
+    auto segment = [&](int s) {
+        const void* pa[1] = {a.A[a.nseg > 1 ? s : z]};
+        const int64_t la[1] = {a.lda};
+        oa.init(pa, la, m0, a.M, a.K, wave, lane);
+        const void* pb[2] = {a.B[HALVES == 2 ? 0 : a.nseg > 1 ? s : z], a.B[1]};
+        const int64_t lb[2] = {a.ldb[HALVES == 2 ? 0 : a.nseg > 1 ? s : z], a.ldb[1]};
+        ob.init(pb, lb, n0, a.N, a.K, wave, lane);
+    };
+    auto load = [&](int step) {
+        if (step == per) segment(1);
+        const int kleft = a.K - (step >= per ? step - per : step) * 64, stage = (step & 1) * STAGE;
+        oa.load(at + stage, wave, lane, kleft, (typename T::E*)(lds + stage));
+        ob.load(at + stage + OA::BYTES, wave, lane, kleft, (typename T::E*)(lds + stage + OA::BYTES));
+    };
+    if (steps) {
+        segment(0);
+        load(0);
+    }
+    for (int step = 0; step < steps; ++step) {
+        // this step's data have arrived, and nobody reads the other buffer any more
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (step + 1 < steps) load(step + 1);
+        const char* sa = lds + (step & 1) * STAGE;
+        const char* sb = sa + OA::BYTES;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            s8 fa[FM], fb[FN];
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+                fb[j] = OB::fragment(sb, HALVES == 2 ? (j / (FN / 2)) * NT + wn * (NT / NWN) + (j % (FN / 2)) * 16 : wn * (BN / NWN) + j * 16, kk, lane);
+#pragma unroll
+            for (int i = 0; i < FM; ++i) fa[i] = OA::fragment(sa, wm * (BM / NWM) + i * 16, kk, lane);
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = T::mfma(fb[j], fa[i], acc[i][j]);
+        }
+    }
+    const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int m = m0 + wm * (BM / NWM) + i * 16 + r;
+        if (m >= a.M) continue;
+        if constexpr (EPI == EPI_GATE)
+#pragma unroll
+            for (int j = 0; j < FN / 2; ++j) finish<T, EPI>(a, 0, m, n0 + wn * (NT / NWN) + j * 16 + g * 4, acc[i][j], acc[i][j + FN / 2]);
+        else
+#pragma unroll
+            for (int j = 0; j < FN; ++j) finish<T, EPI>(a, z, m, n0 + wn * (BN / NWN) + j * 16 + g * 4, acc[i][j], f4{});
     }
 }
 

@@ -41,30 +41,51 @@ int misaligned(const void* p, int e) { return (uintptr_t)p % e != 0; }
 
 int vec(const void* p, int64_t ld, int e) { return (uintptr_t)p % 16 == 0 && ld * e % 16 == 0; }
 
+// a row of 16-bit elements starts on a 4-byte boundary, and a tile's offsets fit 31 bits
+bool tileable(const void* p, int64_t ld) { return (uintptr_t)p % 4 == 0 && ld % 2 == 0 && ld < (1 << 22); }
+
 template <class T, int EPI, bool AK, bool BKc>
-int launch3(ude_ctx* c, const Args& a, int batch) {
-    const int64_t tiles = (int64_t)((a.M + 63) / 64) * ((a.N + (EPI == EPI_GATE ? 31 : 63)) / (EPI == EPI_GATE ? 32 : 64));
-    if (tiles >= 1 << 24) return fail(c, UDE_ERR_UNSUPPORTED, "gated_ffn: %lld tiles", (long long)tiles);
-    hipLaunchKernelGGL((gemm_any<T, EPI, AK, BKc>), dim3((unsigned)tiles, 1, batch), dim3(256), 0, c->stream, a);
+int launch3(ude_ctx* c, const Args& a, int batch, bool tile) {
+    constexpr int H = EPI == EPI_GATE ? 2 : 1;
+    auto tiles = [&](int bm, int bn) { return (int64_t)((a.M + bm - 1) / bm) * ((a.N + bn / H - 1) / (bn / H)); };
+    if constexpr (sizeof(typename T::E) == 2) {
+        if (tile && tiles(128, 128) < 1 << 22) {
+            if (tiles(256, 256) * batch >= 128)
+                hipLaunchKernelGGL((gemm_tile<T, EPI, AK, BKc, 256, 256, 2, 4>), dim3((unsigned)tiles(256, 256), 1, batch), dim3(512), 0, c->stream, a);
+            else
+                hipLaunchKernelGGL((gemm_tile<T, EPI, AK, BKc, 128, 128, 2, 2>), dim3((unsigned)tiles(128, 128), 1, batch), dim3(256), 0, c->stream, a);
+            HIPCHK(c, hipGetLastError());
+            return UDE_OK;
+        }
+    }
+    const int64_t n = tiles(64, 64);
+    if (n >= 1 << 24) return fail(c, UDE_ERR_UNSUPPORTED, "gated_ffn: %lld tiles", (long long)n);
+    hipLaunchKernelGGL((gemm_any<T, EPI, AK, BKc>), dim3((unsigned)n, 1, batch), dim3(256), 0, c->stream, a);
     HIPCHK(c, hipGetLastError());
     return UDE_OK;
 }
 template <class T, int EPI>
-int launch2(ude_ctx* c, const Args& a, bool ak, bool bk, int batch) {
-    return ak ? (bk ? launch3<T, EPI, true, true>(c, a, batch) : launch3<T, EPI, true, false>(c, a, batch))
-              : (bk ? launch3<T, EPI, false, true>(c, a, batch) : launch3<T, EPI, false, false>(c, a, batch));
+int launch2(ude_ctx* c, const Args& a, bool ak, bool bk, int batch, bool tile) {
+    if constexpr (EPI == EPI_STORE)
+        if (!ak) return bk ? fail(c, UDE_ERR_INVALID, "gated_ffn: operand orders") : launch3<T, EPI, false, false>(c, a, batch, tile);
+    return bk ? launch3<T, EPI, true, true>(c, a, batch, tile) : launch3<T, EPI, true, false>(c, a, batch, tile);
 }
 template <int EPI>
 int launch(ude_ctx* c, int dtype, Args a, bool ak, bool bk, int batch = 1) {
     const int e = esize(dtype);
-    a.vecA = a.vecB = 1;
+    a.vecA = a.vecB = a.vecC = 1;
+    bool tile = true;
     for (int i = 0; i < 2; ++i) {
         if (a.A[i] && !vec(a.A[i], a.lda, e)) a.vecA = 0;
         if (a.B[i] && !vec(a.B[i], a.ldb[i], e)) a.vecB = 0;
+        if (a.C[i] && ((uintptr_t)a.C[i] % (4 * e) || a.ldc[i] % 4)) a.vecC = 0;
+        tile = tile && (!a.A[i] || tileable(a.A[i], a.lda)) && (!a.B[i] || tileable(a.B[i], a.ldb[i]));
     }
-    if (dtype == UDE_DT_F32) return launch2<F32, EPI>(c, a, ak, bk, batch);
-    if (dtype == UDE_DT_F16) return launch2<F16, EPI>(c, a, ak, bk, batch);
-    return launch2<BF16, EPI>(c, a, ak, bk, batch);
+    // gate and up are rows of N floats; dg, du, h lie in the workspace, rows of a multiple of 8
+    if (EPI != EPI_STORE && a.gate && (a.N % 4 || (uintptr_t)a.gate % 16 || (uintptr_t)a.up % 16)) a.vecC = 0;
+    if (dtype == UDE_DT_F32) return launch2<F32, EPI>(c, a, ak, bk, batch, false);
+    if (dtype == UDE_DT_F16) return launch2<F16, EPI>(c, a, ak, bk, batch, tile);
+    return launch2<BF16, EPI>(c, a, ak, bk, batch, tile);
 }
 
 }  // namespace
