@@ -285,8 +285,8 @@ static __device__ inline i4 records(const char* base, int64_t bytes) {
     r[3] = 0x00020000;
     return r;
 }
-static __device__ inline void to_lds(unsigned at, unsigned off, i4 r) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(r) : "m0");
+static __device__ inline void to_lds(unsigned at, unsigned off, i4 r, unsigned from) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(at), "v"(off), "s"(r), "s"(from) : "m0");
 }
 static __device__ inline unsigned lds_address(const void* p) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p; }
 
@@ -304,23 +304,18 @@ struct Operand {
     static constexpr int BYTES = ROWS * 128;
     static_assert(N * 8 * NW == ROWS && N % HALVES == 0, "pieces");
     const char* base[HALVES];
-    int64_t left[HALVES], step[HALVES];
+    i4 rec[HALVES];
+    unsigned step[HALVES];  // bytes of 64 k
     unsigned off[N];
     int koff;  // "K": first k of this lane's chunks; "R": not used
 
-    // rows row0.. of matrices with `rows` rows and K columns
-    __device__ inline void init(const void* const* p, const int64_t* ld, int row0, int rows, int K, int wave, int lane) {
+    // columns k0.. of rows row0.. of matrices with `rows` rows and K columns
+    __device__ inline void init(const void* const* p, const int64_t* ld, int row0, int rows, int k0, int K, int wave, int lane) {
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
-            if constexpr (KC) {
-                base[h] = (const char*)p[h] + (int64_t)row0 * ld[h] * 2;
-                left[h] = ((int64_t)(rows - 1 - row0) * ld[h] + K) * 2;
-                step[h] = 128;
-            } else {
-                base[h] = (const char*)p[h] + (int64_t)row0 * 2;
-                left[h] = ((int64_t)(K - 1) * ld[h] + rows - row0) * 2;
-                step[h] = 128 * ld[h];
-            }
+            base[h] = (const char*)p[h] + (KC ? (int64_t)row0 * ld[h] + k0 : (int64_t)k0 * ld[h] + row0) * 2;
+            rec[h] = records(base[h], (KC ? (int64_t)(rows - 1 - row0) * ld[h] + K - k0 : (int64_t)(K - 1 - k0) * ld[h] + rows - row0) * 2);
+            step[h] = KC ? 128 : 128 * (unsigned)ld[h];
         }
         koff = 0;
 #pragma unroll
@@ -338,33 +333,29 @@ struct Operand {
             }
         }
     }
-    // issues the loads of one step to LDS at `at`, then moves on; kleft = columns from this step on
-    __device__ inline void load(unsigned at, int wave, int lane, int kleft, E* lds) {
-        i4 r[HALVES];
+    // piece i of the whole step n to LDS at `at`
+    __device__ inline void piece(int i, unsigned at, int wave, int n) {
+        const int h = i / (N / HALVES);
+        to_lds(at + (i * NW + wave) * 1024, off[i], rec[h], n * step[h]);
+    }
+    // a last step of kleft < 64 k, `n` steps behind k0; where 8 does not divide kleft, a "K" operand goes element by element
+    __device__ inline void tail(unsigned at, int wave, int lane, int n, int kleft, char* lds) {
+        if (!KC || kleft % 8 == 0) {
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h) r[h] = records(base[h], left[h]);
-        const bool full = !KC || kleft >= 64;
-        if (full || kleft % 8 == 0) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const unsigned o = full || koff < kleft ? off[i] : OUTSIDE;
-                to_lds(at + (i * NW + wave) * 1024, o, r[i / (N / HALVES)]);
-            }
-        } else {  // the last step of a K that 8 does not divide: element by element
+            for (int i = 0; i < N; ++i) to_lds(at + (i * NW + wave) * 1024, !KC || koff < kleft ? off[i] : OUTSIDE, rec[i / (N / HALVES)], n * step[i / (N / HALVES)]);
+        } else {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 s8 v = {};
                 if (off[i] != OUTSIDE) {
-                    const E* p = (const E*)(base[i / (N / HALVES)] + off[i]);
+                    const E* p = (const E*)(base[i / (N / HALVES)] + off[i] + n * step[i / (N / HALVES)]);
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
                         if (koff + e < kleft) v[e] = p[e];
                 }
-                *(s8*)((char*)lds + (i * NW + wave) * 1024 + lane * 16) = v;
+                *(s8*)(lds + (i * NW + wave) * 1024 + lane * 16) = v;
             }
         }
-#pragma unroll
-        for (int h = 0; h < HALVES; ++h) base[h] += step[h], left[h] -= step[h];
     }
     // the 8 k of row `row` (a multiple of 16, plus lane & 15) that a lane feeds to the matrix instruction of k-half kk
     static __device__ inline s8 fragment(const char* lds, int row, int kk, int lane) {
@@ -381,8 +372,8 @@ struct Operand {
     }
 };
 
-template <class T, int EPI, bool AK, bool BKc, int BM, int BN, int NWM, int NWN>
-__global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(2, 2))) void gemm_tile(const Args a) {
+template <class T, int EPI, bool AK, bool BKc, int BM, int BN, int NWM, int NWN, int OCC>
+__global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void gemm_tile(const Args a) {
     constexpr int NW = NWM * NWN, FM = BM / NWM / 16, FN = BN / NWN / 16, HALVES = EPI == EPI_GATE ? 2 : 1;
     constexpr int NT = BN / HALVES;  // output columns of a tile
     typedef Operand<T, AK, BM, NW, 1> OA;
@@ -404,59 +395,132 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
     const int m0 = (gm0 + (t - group * GM * nn) % gsize) * BM, n0 = (t - group * GM * nn) / gsize * NT;
 
     f4 acc[FM][FN] = {};
+    s8 fa[2][FM], fb[2][FN];
     OA oa;
     OB ob;
     const unsigned at = __builtin_amdgcn_readfirstlane(lds_address(lds));
-    const int per = (a.K + 63) / 64, steps = per * a.nseg;
-    auto segment = [&](int s) {
-        const void* pa[1] = {a.A[a.nseg > 1 ? s : z]};
-        const int64_t la[1] = {a.lda};
-        oa.init(pa, la, m0, a.M, a.K, wave, lane);
-        const void* pb[2] = {a.B[HALVES == 2 ? 0 : a.nseg > 1 ? s : z], a.B[1]};
-        const int64_t lb[2] = {a.ldb[HALVES == 2 ? 0 : a.nseg > 1 ? s : z], a.ldb[1]};
-        ob.init(pb, lb, n0, a.N, a.K, wave, lane);
+    auto read_a = [&](int i, int kk, const char* stage) { return OA::fragment(stage, wm * (BM / NWM) + i * 16, kk, lane); };
+    auto read_b = [&](int j, int kk, const char* stage) {
+        return OB::fragment(stage + OA::BYTES, HALVES == 2 ? (j / (FN / 2)) * NT + wn * (NT / NWN) + (j % (FN / 2)) * 16 : wn * (BN / NWN) + j * 16, kk, lane);
     };
-    auto load = [&](int step) {
-        if (step == per) segment(1);
-        const int kleft = a.K - (step >= per ? step - per : step) * 64, stage = (step & 1) * STAGE;
-        oa.load(at + stage, wave, lane, kleft, (typename T::E*)(lds + stage));
-        ob.load(at + stage + OA::BYTES, wave, lane, kleft, (typename T::E*)(lds + stage + OA::BYTES));
+    auto load = [&](int stage, int n) {
+#pragma unroll
+        for (int i = 0; i < OA::N; ++i) oa.piece(i, at + stage, wave, n);
+#pragma unroll
+        for (int i = 0; i < OB::N; ++i) ob.piece(i, at + stage + OA::BYTES, wave, n);
     };
-    if (steps) {
-        segment(0);
-        load(0);
-    }
-    for (int step = 0; step < steps; ++step) {
-        // this step's data have arrived, and nobody reads the other buffer any more
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (step + 1 < steps) load(step + 1);
-        const char* sa = lds + (step & 1) * STAGE;
-        const char* sb = sa + OA::BYTES;
+    // rows of products are the grain that reads and loads are dealt out over; the compiler keeps the order of the grains
+    auto reads = [&](int i, int half, const char* stage) {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            s8 fa[FM], fb[FN];
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-                fb[j] = OB::fragment(sb, HALVES == 2 ? (j / (FN / 2)) * NT + wn * (NT / NWN) + (j % (FN / 2)) * 16 : wn * (BN / NWN) + j * 16, kk, lane);
-#pragma unroll
-            for (int i = 0; i < FM; ++i) fa[i] = OA::fragment(sa, wm * (BM / NWM) + i * 16, kk, lane);
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = T::mfma(fb[j], fa[i], acc[i][j]);
+        for (int r = 0; r < FM + FN; ++r) {
+            if (r * 3 * FM / (4 * (FM + FN)) != i) continue;  // all of them in the first three quarters
+            if (r < FN)
+                fb[half][r] = read_b(r, half, stage);
+            else
+                fa[half][r - FN] = read_a(r - FN, half, stage);
         }
-    }
-    const int r = lane & 15, g = lane >> 4;
+    };
+    // step n, whose first half is in registers, out of `here`; leaves step n + 1's first half there and loads step `to` into `here`
+    auto body = [&](int here, int to) {
+        const char* from = lds + here;
+        const char* next = lds + STAGE - here;
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-        const int m = m0 + wm * (BM / NWM) + i * 16 + r;
-        if (m >= a.M) continue;
-        if constexpr (EPI == EPI_GATE)
+        for (int i = 0; i < FM; ++i) {
+            reads(i, 1, from);
 #pragma unroll
-            for (int j = 0; j < FN / 2; ++j) finish<T, EPI>(a, 0, m, n0 + wn * (NT / NWN) + j * 16 + g * 4, acc[i][j], acc[i][j + FN / 2]);
-        else
+            for (int j = 0; j < FN; ++j) acc[i][j] = T::mfma(fb[0][j], fa[0][i], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // the next step's data have arrived, and nobody reads this step's buffer any more
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < FN; ++j) finish<T, EPI>(a, z, m, n0 + wn * (BN / NWN) + j * 16 + g * 4, acc[i][j], f4{});
+        for (int i = 0; i < FM; ++i) {
+#pragma unroll
+            for (int p = i * OA::N / FM; p < (i + 1) * OA::N / FM; ++p) oa.piece(p, at + here, wave, to);
+#pragma unroll
+            for (int p = i * OB::N / FM; p < (i + 1) * OB::N / FM; ++p) ob.piece(p, at + here + OA::BYTES, wave, to);
+            reads(i, 0, next);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = T::mfma(fb[1][j], fa[1][i], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // Offsets within a run of steps stay below 2^31: a run of an "R" operand with long rows is shorter than K
+    int64_t most = 1 << 24;
+    if (!AK && (1 << 30) / (128 * a.lda) < most) most = (1 << 30) / (128 * a.lda);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        if (!BKc && a.ldb[h] && (1 << 30) / (128 * a.ldb[h]) < most) most = (1 << 30) / (128 * a.ldb[h]);
+    const int run = (int)most;
+    for (int seg = 0; seg < a.nseg; ++seg)
+        for (int64_t k0 = 0; k0 < a.K; k0 += (int64_t)run * 64) {
+            {
+                const int sa = a.nseg > 1 ? seg : z, sb = HALVES == 2 ? 0 : sa;
+                const void* pa[1] = {a.A[sa]};
+                const int64_t la[1] = {a.lda};
+                oa.init(pa, la, m0, a.M, (int)k0, a.K, wave, lane);
+                const void* pb[2] = {a.B[sb], a.B[1]};
+                const int64_t lb[2] = {a.ldb[sb], a.ldb[1]};
+                ob.init(pb, lb, n0, a.N, (int)k0, a.K, wave, lane);
+            }
+            const int left = (int)((a.K - k0) / 64), full = left < run ? left : run, rest = left < run ? (int)((a.K - k0) % 64) : 0;
+            if (full) {
+                // (where no step is left to load, the last one is loaded again, into a buffer that is not read)
+                load(0, 0);
+                load(STAGE, full > 1);
+                asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(OA::N + OB::N) : "memory");
+#pragma unroll
+                for (int j = 0; j < FN; ++j) fb[0][j] = read_b(j, 0, lds);
+#pragma unroll
+                for (int i = 0; i < FM; ++i) fa[0][i] = read_a(i, 0, lds);
+                for (int n = 0; n < full; n += 2) {
+                    body(0, n + 2 < full ? n + 2 : full - 1);
+                    if (n + 1 < full) body(STAGE, n + 3 < full ? n + 3 : full - 1);
+                }
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            }
+            if (rest) {
+                oa.tail(at, wave, lane, full, rest, lds);
+                ob.tail(at + OA::BYTES, wave, lane, full, rest, lds + OA::BYTES);
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk) {
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) fb[0][j] = read_b(j, kk, lds);
+#pragma unroll
+                    for (int i = 0; i < FM; ++i) fa[0][i] = read_a(i, kk, lds);
+#pragma unroll
+                    for (int i = 0; i < FM; ++i)
+#pragma unroll
+                        for (int j = 0; j < FN; ++j) acc[i][j] = T::mfma(fb[0][j], fa[0][i], acc[i][j]);
+                }
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            }
+        }
+    // epilogue: 32 rows of a wavefront at a time through LDS, so that the code of finish() stands in a loop and a row's lanes store side by
+    // side.  (The rows are four floats longer than they need to be: 8 lanes that write 16 bytes of 8 rows touch every bank once.)
+    constexpr int COLS = BN / NWN, LDC = COLS + 4, CT = COLS / HALVES;
+    static_assert(NW * 32 * LDC * 4 <= 2 * STAGE, "epilogue");
+    float* mine = (float*)lds + wave * 32 * LDC;
+#pragma unroll
+    for (int p = 0; p < FM / 2; ++p) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) *(f4*)(mine + (i * 16 + (lane & 15)) * LDC + j * 16 + (lane >> 4) * 4) = acc[2 * p + i][j];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll 1
+        for (int e = lane; e < 32 * CT / 4; e += 64) {
+            const int row = e / (CT / 4), col = e % (CT / 4) * 4, m = m0 + wm * (BM / NWM) + p * 32 + row;
+            if (m >= a.M) break;
+            const f4 c = *(const f4*)(mine + row * LDC + col);
+            if constexpr (EPI == EPI_GATE)
+                finish<T, EPI>(a, 0, m, n0 + wn * CT + col, c, *(const f4*)(mine + row * LDC + CT + col));
+            else
+                finish<T, EPI>(a, z, m, n0 + wn * CT + col, c, f4{});
+        }
     }
 }
 

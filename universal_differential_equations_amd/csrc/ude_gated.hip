@@ -51,9 +51,9 @@ int launch3(ude_ctx* c, const Args& a, int batch, bool tile) {
     if constexpr (sizeof(typename T::E) == 2) {
         if (tile && tiles(128, 128) < 1 << 22) {
             if (tiles(256, 256) * batch >= 128)
-                hipLaunchKernelGGL((gemm_tile<T, EPI, AK, BKc, 256, 256, 2, 4>), dim3((unsigned)tiles(256, 256), 1, batch), dim3(512), 0, c->stream, a);
+                hipLaunchKernelGGL((gemm_tile<T, EPI, AK, BKc, 256, 256, 2, 2, 1>), dim3((unsigned)tiles(256, 256), 1, batch), dim3(256), 0, c->stream, a);
             else
-                hipLaunchKernelGGL((gemm_tile<T, EPI, AK, BKc, 128, 128, 2, 2>), dim3((unsigned)tiles(128, 128), 1, batch), dim3(256), 0, c->stream, a);
+                hipLaunchKernelGGL((gemm_tile<T, EPI, AK, BKc, 128, 128, 2, 2, 2>), dim3((unsigned)tiles(128, 128), 1, batch), dim3(256), 0, c->stream, a);
             HIPCHK(c, hipGetLastError());
             return UDE_OK;
         }
