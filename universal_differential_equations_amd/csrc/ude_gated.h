@@ -263,8 +263,8 @@ __global__ __launch_bounds__(256) void gemm_any(const Args a) {
 }
 
 // ---- the tile kernel of the 16-bit kinds ------------------------------------------------------------------------------------------
-// A BM x BN tile of C by NWM x NWN wavefronts; K in steps of 64 through two LDS buffers that buffer_load .. lds fills 16 bytes a lane,
-// straight from memory: while step k is multiplied, step k + 1 is on its way.  What a descriptor's record count does not cover is
+// A BM x BN tile of C by NWM x NWN wavefronts; K in steps of 64 through LDS buffers that buffer_load .. lds fills 16 bytes a lane,
+// straight from memory: while step k is multiplied, the next ones are on their way.  What a descriptor's record count does not cover is
 // filled with zeros, so that edges cost no branches; a lane outside asks for OUTSIDE.
 //
 // LDS layouts (a 1 KB piece is one instruction of one wavefront, lane l at 16 l):
@@ -378,8 +378,8 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
     constexpr int NT = BN / HALVES;  // output columns of a tile
     typedef Operand<T, AK, BM, NW, 1> OA;
     typedef Operand<T, BKc, BN, NW, HALVES> OB;
-    constexpr int STAGE = OA::BYTES + OB::BYTES;
-    __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+    constexpr int BUFFERS = 2 * OB::BYTES + 3 * OA::BYTES;  // two of B, then three of A
+    __shared__ __attribute__((aligned(1024))) char lds[BUFFERS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % NWM, wn = wave / NWM;
     const int z = blockIdx.z;
     // workgroup b runs on XCD b % 8: each XCD takes a contiguous run of tiles, in groups of 8 rows of tiles, so that its L2 holds the
@@ -399,53 +399,60 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
     OA oa;
     OB ob;
     const unsigned at = __builtin_amdgcn_readfirstlane(lds_address(lds));
-    auto read_a = [&](int i, int kk, const char* stage) { return OA::fragment(stage, wm * (BM / NWM) + i * 16, kk, lane); };
-    auto read_b = [&](int j, int kk, const char* stage) {
-        return OB::fragment(stage + OA::BYTES, HALVES == 2 ? (j / (FN / 2)) * NT + wn * (NT / NWN) + (j % (FN / 2)) * 16 : wn * (BN / NWN) + j * 16, kk, lane);
+    auto read_a = [&](int i, int kk, int stage) { return OA::fragment(lds + stage, wm * (BM / NWM) + i * 16, kk, lane); };
+    auto read_b = [&](int j, int kk, int stage) {
+        return OB::fragment(lds + stage, HALVES == 2 ? (j / (FN / 2)) * NT + wn * (NT / NWN) + (j % (FN / 2)) * 16 : wn * (BN / NWN) + j * 16, kk, lane);
     };
-    auto load = [&](int stage, int n) {
+    auto load_a = [&](int stage, int n) {
 #pragma unroll
         for (int i = 0; i < OA::N; ++i) oa.piece(i, at + stage, wave, n);
+    };
+    auto load_b = [&](int stage, int n) {
 #pragma unroll
-        for (int i = 0; i < OB::N; ++i) ob.piece(i, at + stage + OA::BYTES, wave, n);
+        for (int i = 0; i < OB::N; ++i) ob.piece(i, at + stage, wave, n);
     };
     // rows of products are the grain that reads and loads are dealt out over; the compiler keeps the order of the grains
-    auto reads = [&](int i, int half, const char* stage) {
+    auto reads = [&](int i, int half, int sa, int sb) {
 #pragma unroll
         for (int r = 0; r < FM + FN; ++r) {
             if (r * 3 * FM / (4 * (FM + FN)) != i) continue;  // all of them in the first three quarters
             if (r < FN)
-                fb[half][r] = read_b(r, half, stage);
+                fb[half][r] = read_b(r, half, sb);
             else
-                fa[half][r - FN] = read_a(r - FN, half, stage);
+                fa[half][r - FN] = read_a(r - FN, half, sa);
         }
     };
-    // step n, whose first half is in registers, out of `here`; leaves step n + 1's first half there and loads step `to` into `here`
-    auto body = [&](int here, int to) {
-        const char* from = lds + here;
-        const char* next = lds + STAGE - here;
+    // Step n, whose first half is in registers, out of the buffers sa and sb; leaves the first half of step n + 1 there, starts the loads of
+    // B's step n + 2 and of A's step n + 3.  (The loads of a step take about as long to issue as half a step's products: A's third buffer
+    // lets the later half of them arrive a step later.)
+    auto body = [&](int sa, int sa1, int sb, int n, int last) {
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
-            reads(i, 1, from);
+            reads(i, 1, sa, sb);
 #pragma unroll
             for (int j = 0; j < FN; ++j) acc[i][j] = T::mfma(fb[0][j], fa[0][i], acc[i][j]);
             __builtin_amdgcn_sched_barrier(0);
         }
-        // the next step's data have arrived, and nobody reads this step's buffer any more
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        // step n + 1 has arrived but for what A's loads brought for n + 2, and nobody reads this step's buffers any more
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(OA::N) : "memory");
         __builtin_amdgcn_sched_barrier(0);
+        // (where no step is left to load, the last one is loaded again, into a buffer that is not read)
+        const int nb = n + 2 < last ? n + 2 : last, na = n + 3 < last ? n + 3 : last;
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
 #pragma unroll
-            for (int p = i * OA::N / FM; p < (i + 1) * OA::N / FM; ++p) oa.piece(p, at + here, wave, to);
-#pragma unroll
-            for (int p = i * OB::N / FM; p < (i + 1) * OB::N / FM; ++p) ob.piece(p, at + here + OA::BYTES, wave, to);
-            reads(i, 0, next);
+            for (int p = i * (OA::N + OB::N) / FM; p < (i + 1) * (OA::N + OB::N) / FM; ++p)
+                if (p < OB::N)
+                    ob.piece(p, at + sb, wave, nb);
+                else
+                    oa.piece(p - OB::N, at + sa, wave, na);
+            reads(i, 0, sa1, OB::BYTES - sb);
 #pragma unroll
             for (int j = 0; j < FN; ++j) acc[i][j] = T::mfma(fb[1][j], fa[1][i], acc[i][j]);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
+    constexpr int A0 = 2 * OB::BYTES, A1 = A0 + OA::BYTES, A2 = A1 + OA::BYTES;
     // Offsets within a run of steps stay below 2^31: a run of an "R" operand with long rows is shorter than K
     int64_t most = 1 << 24;
     if (!AK && (1 << 30) / (128 * a.lda) < most) most = (1 << 30) / (128 * a.lda);
@@ -466,30 +473,34 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
             }
             const int left = (int)((a.K - k0) / 64), full = left < run ? left : run, rest = left < run ? (int)((a.K - k0) % 64) : 0;
             if (full) {
-                // (where no step is left to load, the last one is loaded again, into a buffer that is not read)
-                load(0, 0);
-                load(STAGE, full > 1);
-                asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(OA::N + OB::N) : "memory");
+                const int last = full - 1;
+                load_a(A0, 0), load_b(0, 0);
+                load_a(A1, 1 < last ? 1 : last), load_b(OB::BYTES, 1 < last ? 1 : last);
+                load_a(A2, 2 < last ? 2 : last);
+                asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * OA::N + OB::N) : "memory");
 #pragma unroll
-                for (int j = 0; j < FN; ++j) fb[0][j] = read_b(j, 0, lds);
+                for (int j = 0; j < FN; ++j) fb[0][j] = read_b(j, 0, 0);
 #pragma unroll
-                for (int i = 0; i < FM; ++i) fa[0][i] = read_a(i, 0, lds);
+                for (int i = 0; i < FM; ++i) fa[0][i] = read_a(i, 0, A0);
+                int s0 = A0, s1 = A1, s2 = A2;
                 for (int n = 0; n < full; n += 2) {
-                    body(0, n + 2 < full ? n + 2 : full - 1);
-                    if (n + 1 < full) body(STAGE, n + 3 < full ? n + 3 : full - 1);
+                    body(s0, s1, 0, n, last);
+                    if (n + 1 < full) body(s1, s2, OB::BYTES, n + 1, last);
+                    const int s = s0;
+                    s0 = s2, s2 = s1, s1 = s;
                 }
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             }
             if (rest) {
-                oa.tail(at, wave, lane, full, rest, lds);
-                ob.tail(at + OA::BYTES, wave, lane, full, rest, lds + OA::BYTES);
+                oa.tail(at + A0, wave, lane, full, rest, lds + A0);
+                ob.tail(at, wave, lane, full, rest, lds);
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk) {
 #pragma unroll
-                    for (int j = 0; j < FN; ++j) fb[0][j] = read_b(j, kk, lds);
+                    for (int j = 0; j < FN; ++j) fb[0][j] = read_b(j, kk, 0);
 #pragma unroll
-                    for (int i = 0; i < FM; ++i) fa[0][i] = read_a(i, kk, lds);
+                    for (int i = 0; i < FM; ++i) fa[0][i] = read_a(i, kk, A0);
 #pragma unroll
                     for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -501,7 +512,7 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
     // epilogue: 32 rows of a wavefront at a time through LDS, so that the code of finish() stands in a loop and a row's lanes store side by
     // side.  (The rows are four floats longer than they need to be: 8 lanes that write 16 bytes of 8 rows touch every bank once.)
     constexpr int COLS = BN / NWN, LDC = COLS + 4, CT = COLS / HALVES;
-    static_assert(NW * 32 * LDC * 4 <= 2 * STAGE, "epilogue");
+    static_assert(NW * 32 * LDC * 4 <= BUFFERS, "epilogue");
     float* mine = (float*)lds + wave * 32 * LDC;
 #pragma unroll
     for (int p = 0; p < FM / 2; ++p) {
