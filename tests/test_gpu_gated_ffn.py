@@ -98,6 +98,20 @@ def test_many_large_tiles(size, kind):
         check(*made(*size, kind, rows, seed=15))
 
 
+@pytest.mark.parametrize("size", [(1, 4096, 1408, 512), (24, 1000, 2730, 264), (32, 2048, 512, 4100), (33, 72, 5000, 136), (200, 136, 3000, 80), (3000, 72, 136, 264), (600, 2056, 72, 1032)],
+                         ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("kind", KINDS[:2], ids=IDS[:2])
+def test_products_cut_along_k(size, kind):
+    """few tiles and a long inner axis: parts of K, some of them across the two halves of dx's product, some empty; the same bits twice"""
+    import universal_differential_equations_amd as U
+    for rows in (True, False):
+        s = made(*size, kind, rows, seed=16)
+        got = check(*s)
+        y, saved = U.gated_ffn(*s[:4], save=True)
+        again = dict(zip(("dx", "dwg", "dwu", "dwd"), U.gated_ffn_pullback(saved, s[4])), y=y)
+        assert all(torch.equal(got[k], again[k]) for k in again)
+
+
 def test_against_differences():
     """directional derivatives of sum(y * c) by central differences of the Float64 statement"""
     import universal_differential_equations_amd as U

@@ -44,63 +44,90 @@ struct BF16 {
     }
 };
 
-// act(g) and act'(g) in Float32
-static __device__ inline float gate_act(int act, float g, float* slope) {
-    switch (act) {
-        case UDE_GATE_TANH: {
-            const float t = tanhf(g);
-            *slope = 1.f - t * t;
-            return t;
-        }
-        case UDE_GATE_RBF: {
-            const float e = expf(-g * g);
-            *slope = -2.f * g * e;
-            return e;
-        }
-        case UDE_GATE_RELU:
-            *slope = g > 0.f ? 1.f : 0.f;
-            return g > 0.f ? g : g * 0.f;  // (NaN stays NaN)
-        case UDE_GATE_SIGMOID: {
-            const float s = 1.f / (1.f + expf(-g));
-            *slope = s * (1.f - s);
-            return s;
-        }
-        case UDE_GATE_SWISH: {
-            const float s = 1.f / (1.f + expf(-g));
-            *slope = s * (1.f + g * (1.f - s));
-            return g * s;
-        }
-        case UDE_GATE_GELU_TANH: {
-            const float c = 0.7978845608028654f, q = 0.044715f;
-            const float t = tanhf(c * (g + q * g * g * g));
-            *slope = 0.5f * (1.f + t) + 0.5f * g * (1.f - t * t) * c * (1.f + 3.f * q * g * g);
-            return 0.5f * g * (1.f + t);
-        }
-        case UDE_GATE_GELU_ERF: {
-            const float p = 0.5f * (1.f + erff(g * 0.7071067811865476f));
-            *slope = p + g * 0.3989422804014327f * expf(-0.5f * g * g);
-            return g * p;
-        }
-        default:
-            *slope = 1.f;
-            return g;
+// act(g) and act'(g) in Float32.  QUICK (16-bit kinds): the hardware's exponential and reciprocal, a few 2^-22 of the value off, far below
+// the rounding of the result; Float32 calls the accurate functions.  Sums that would cancel are written as what they are equal to:
+// (1 + tanh z) / 2 = sigmoid(2 z), (1 + erf z) / 2 = erfc(-z) / 2.
+template <bool QUICK>
+static __device__ inline float sigmoid(float x) {
+    return QUICK ? __builtin_amdgcn_rcpf(1.f + __expf(-x)) : 1.f / (1.f + expf(-x));
+}
+template <bool QUICK, int ACT>
+static __device__ inline float gate_act(float g, float* slope) {
+    if constexpr (ACT == UDE_GATE_TANH) {
+        const float t = tanhf(g);
+        *slope = 1.f - t * t;
+        return t;
+    } else if constexpr (ACT == UDE_GATE_RBF) {
+        const float e = QUICK ? __expf(-g * g) : expf(-g * g);
+        *slope = -2.f * g * e;
+        return e;
+    } else if constexpr (ACT == UDE_GATE_RELU) {
+        *slope = g > 0.f ? 1.f : 0.f;
+        return g > 0.f ? g : g * 0.f;  // (NaN stays NaN)
+    } else if constexpr (ACT == UDE_GATE_SIGMOID) {
+        const float s = sigmoid<QUICK>(g);
+        *slope = s * (1.f - s);
+        return s;
+    } else if constexpr (ACT == UDE_GATE_SWISH) {
+        const float s = sigmoid<QUICK>(g);
+        *slope = s * (1.f + g * (1.f - s));
+        return g * s;
+    } else if constexpr (ACT == UDE_GATE_GELU_TANH) {
+        const float c = 1.5957691216057308f, q = 0.044715f;  // 2 sqrt(2 / pi)
+        const float s = sigmoid<QUICK>(c * (g + q * g * g * g));
+        *slope = s + g * s * (1.f - s) * c * (1.f + 3.f * q * g * g);
+        return g * s;
+    } else if constexpr (ACT == UDE_GATE_GELU_ERF) {
+        const float p = 0.5f * erfcf(g * -0.7071067811865476f), x = -0.5f * g * g;
+        *slope = p + g * 0.3989422804014327f * (QUICK ? __expf(x) : expf(x));
+        return g * p;
+    } else {
+        *slope = 1.f;
+        return g;
+    }
+}
+// n values at once, so that the choice of act is made once and the values' chains overlap
+template <bool QUICK, int N, int ACT>
+static __device__ inline void gate_acts(const float* g, float* act, float* slope) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) act[i] = gate_act<QUICK, ACT>(g[i], slope + i);
+}
+template <bool QUICK, int N>
+static __device__ inline void gate_acts(int which, const float* g, float* act, float* slope) {
+    switch (which) {
+        case UDE_GATE_TANH: gate_acts<QUICK, N, UDE_GATE_TANH>(g, act, slope); break;
+        case UDE_GATE_RBF: gate_acts<QUICK, N, UDE_GATE_RBF>(g, act, slope); break;
+        case UDE_GATE_RELU: gate_acts<QUICK, N, UDE_GATE_RELU>(g, act, slope); break;
+        case UDE_GATE_SIGMOID: gate_acts<QUICK, N, UDE_GATE_SIGMOID>(g, act, slope); break;
+        case UDE_GATE_SWISH: gate_acts<QUICK, N, UDE_GATE_SWISH>(g, act, slope); break;
+        case UDE_GATE_GELU_TANH: gate_acts<QUICK, N, UDE_GATE_GELU_TANH>(g, act, slope); break;
+        case UDE_GATE_GELU_ERF: gate_acts<QUICK, N, UDE_GATE_GELU_ERF>(g, act, slope); break;
+        default: gate_acts<QUICK, N, UDE_GATE_IDENTITY>(g, act, slope);
     }
 }
 
 enum { EPI_STORE = 0, EPI_GATE = 1, EPI_PULL = 2 };
 
-struct Args {
-    const void* A[2];
-    const void* B[2];
-    void* C[2];
-    int64_t lda, ldb[2], ldc[2];
-    int M, N, K;
-    int nseg;      // EPI_STORE: products summed into one output, C[0] = sum_s A[s] B[s]^T
-    int act;
+// One product C[m, n] = sum_k A(m, k) B(n, k)
+struct Product {
+    const void *A, *B;
+    void* C;
+    int64_t lda, ldb, ldc;
+    int M, N;
     int vecA, vecB;  // 16-byte loads allowed: base and leading dimension aligned (gemm_any)
     int vecC;        // stores of four consecutive columns allowed
-    float *gate, *up;        // EPI_GATE: stored if not NULL; EPI_PULL: read; leading dimension N
-    void *dg, *du, *h;       // EPI_PULL: dg and du with leading dimension ldc[0], h with ldc[1]
+};
+struct Args {
+    Product p[3];  // EPI_STORE: nprod of them side by side, or (nseg = 2) p[0] + p[1] into p[0].C; EPI_GATE: B of p[0] and p[1]
+    int K, nprod, nseg;
+    int act;
+    // gemm_tile: the tiles from `first` on; quarters: each workgroup a quarter of a 256 x 256 tile; split > 1: each a part of K, the
+    // sums of tile t and part s go to part[(t * split + s) * tile size] and join_parts adds them up
+    int first, quarters, split;
+    float* part;
+    float *gate, *up;     // EPI_GATE: stored if not NULL; EPI_PULL: read; leading dimension N
+    void *dg, *du, *h;    // EPI_PULL: dg and du with leading dimension p[0].ldc, h with ldh
+    int64_t ldh;
 };
 
 // 8 consecutive elements along the stored axis of a tile; elements outside are zero
@@ -120,68 +147,78 @@ static __device__ inline void load8(const E* p, int64_t left, bool row, int vec,
     }
 }
 
-// What a tile kernel does with the four consecutive columns n.. of row m that a lane holds (v = Wu's product for EPI_GATE)
-template <class T, int EPI>
-static __device__ inline void finish(const Args& a, int z, int m, int n, f4 c, f4 v) {
+// What a kernel does with N times four consecutive columns n[].. of rows m[] (v: Wu's products for EPI_GATE)
+template <class T>
+static __device__ inline void store4(typename T::E* to, const float* x, int left, bool vec) {
     typedef typename T::E E;
     typedef E E4 __attribute__((ext_vector_type(4)));
-    if (n >= a.N) return;
-    const int64_t at = (int64_t)m * a.N + n;
-    if constexpr (EPI == EPI_STORE) {
-        E* to = (E*)a.C[z] + (int64_t)m * a.ldc[z] + n;
-        const E4 o = {T::from(c[0]), T::from(c[1]), T::from(c[2]), T::from(c[3])};
-        if (a.vecC && n + 4 <= a.N)
-            *(E4*)to = o;
-        else
+    const E4 o = {T::from(x[0]), T::from(x[1]), T::from(x[2]), T::from(x[3])};
+    if (vec && left >= 4)
+        *(E4*)to = o;
+    else
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (n + q < a.N) to[q] = o[q];
-    } else if constexpr (EPI == EPI_GATE) {
-        E* to = (E*)a.C[0] + (int64_t)m * a.ldc[0] + n;
-        E4 o;
-        float slope;
+        for (int q = 0; q < 4; ++q)
+            if (q < left) to[q] = o[q];
+}
+static __device__ inline void load4(const float* p, float* o, int left, bool vec) {
+    if (vec && left >= 4) {
+        const f4 x = *(const f4*)p;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) o[q] = T::from(gate_act(a.act, c[q], &slope) * v[q]);
-        if (a.vecC && n + 4 <= a.N) {
-            *(E4*)to = o;
-            if (a.gate) {
-                *(f4*)(a.gate + at) = c;
-                *(f4*)(a.up + at) = v;
-            }
-        } else
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (n + q < a.N) {
-                    to[q] = o[q];
-                    if (a.gate) a.gate[at + q] = c[q], a.up[at + q] = v[q];
-                }
+        for (int q = 0; q < 4; ++q) o[q] = x[q];
     } else {
-        const bool four = a.vecC && n + 4 <= a.N;
-        f4 gv = {}, uv = {};
-        if (four)
-            gv = *(const f4*)(a.gate + at), uv = *(const f4*)(a.up + at);
-        else
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (n + q < a.N) gv[q] = a.gate[at + q], uv[q] = a.up[at + q];
-        E4 og, ou, oh;
+        for (int q = 0; q < 4; ++q) o[q] = q < left ? p[q] : 0.f;
+    }
+}
+template <class T, int EPI, int N>
+static __device__ inline void finish(const Args& a, const Product& p, const int* m, const int* n, const f4* c, const f4* v) {
+    typedef typename T::E E;
+    constexpr bool QUICK = sizeof(E) == 2;
+    if constexpr (EPI == EPI_STORE) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            float slope;
-            const float av = gate_act(a.act, gv[q], &slope);
-            og[q] = T::from(c[q] * uv[q] * slope);
-            ou[q] = T::from(c[q] * av);
-            oh[q] = T::from(av * uv[q]);
+        for (int i = 0; i < N; ++i)
+            if (m[i] < p.M && n[i] < p.N) store4<T>((E*)p.C + (int64_t)m[i] * p.ldc + n[i], (const float*)&c[i], p.N - n[i], p.vecC);
+    } else if constexpr (EPI == EPI_GATE) {
+        float act[4 * N], slope[4 * N];
+        gate_acts<QUICK, 4 * N>(a.act, (const float*)c, act, slope);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (m[i] < p.M && n[i] < p.N) {
+                float h[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) h[q] = act[4 * i + q] * v[i][q];
+                store4<T>((E*)p.C + (int64_t)m[i] * p.ldc + n[i], h, p.N - n[i], p.vecC);
+                if (a.gate) {
+                    const int64_t at = (int64_t)m[i] * p.N + n[i];
+                    store4<F32>(a.gate + at, (const float*)&c[i], p.N - n[i], p.vecC);
+                    store4<F32>(a.up + at, (const float*)&v[i], p.N - n[i], p.vecC);
+                }
+            }
+    } else {
+        float g[4 * N], u[4 * N], act[4 * N], slope[4 * N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int64_t at = (int64_t)m[i] * p.N + n[i];
+            const int left = m[i] < p.M ? p.N - n[i] : 0;
+            load4(a.gate + at, g + 4 * i, left, p.vecC);
+            load4(a.up + at, u + 4 * i, left, p.vecC);
         }
-        const int64_t to = (int64_t)m * a.ldc[0] + n, th = (int64_t)m * a.ldc[1] + n;
-        if (four) {
-            *(E4*)((E*)a.dg + to) = og;
-            *(E4*)((E*)a.du + to) = ou;
-            *(E4*)((E*)a.h + th) = oh;
-        } else
+        gate_acts<QUICK, 4 * N>(a.act, g, act, slope);
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (n + q < a.N) ((E*)a.dg)[to + q] = og[q], ((E*)a.du)[to + q] = ou[q], ((E*)a.h)[th + q] = oh[q];
+        for (int i = 0; i < N; ++i)
+            if (m[i] < p.M && n[i] < p.N) {
+                float dg[4], du[4], h[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    dg[q] = c[i][q] * u[4 * i + q] * slope[4 * i + q];
+                    du[q] = c[i][q] * act[4 * i + q];
+                    h[q] = act[4 * i + q] * u[4 * i + q];
+                }
+                const int64_t to = (int64_t)m[i] * p.ldc + n[i];
+                store4<T>((E*)a.dg + to, dg, p.N - n[i], p.vecC);
+                store4<T>((E*)a.du + to, du, p.N - n[i], p.vecC);
+                store4<T>((E*)a.h + (int64_t)m[i] * a.ldh + n[i], h, p.N - n[i], p.vecC);
+            }
     }
 }
 
@@ -195,33 +232,36 @@ __global__ __launch_bounds__(256) void gemm_any(const Args a) {
     __shared__ __attribute__((aligned(16))) E sA[BM * LD];
     __shared__ __attribute__((aligned(16))) E sB[BN * LD];
     const int tid = threadIdx.x, lane = tid & 63, wm = (tid >> 6) & 1, wn = tid >> 7;
-    const int nm = (a.M + BM - 1) / BM;
+    const Product& q = a.p[blockIdx.z];
+    const int nm = (q.M + BM - 1) / BM;
+    if ((int)blockIdx.x >= nm * ((q.N + (EPI == EPI_GATE ? BN / 2 : BN) - 1) / (EPI == EPI_GATE ? BN / 2 : BN))) return;  // (the grid is that of the largest)
     constexpr int NT = EPI == EPI_GATE ? BN / 2 : BN;  // output columns of a tile
     const int m0 = (int)(blockIdx.x % nm) * BM, n0 = (int)(blockIdx.x / nm) * NT;
-    const int z = blockIdx.z;
     f4 acc[2][2] = {};
     for (int seg = 0; seg < a.nseg; ++seg) {
-        const E* A = (const E*)a.A[a.nseg > 1 ? seg : z];
-        const int bi = a.nseg > 1 ? seg : z;
+        const Product& s = a.p[a.nseg > 1 ? seg : blockIdx.z];
+        const E* A = (const E*)s.A;
         for (int k0 = 0; k0 < a.K; k0 += KS) {
             E va[8], vb[8];
             int ra, ka, rb, kb;
             if (AK) {
                 ra = tid >> 2, ka = (tid & 3) * 8;
-                load8(A + (int64_t)(m0 + ra) * a.lda + k0 + ka, a.K - k0 - ka, m0 + ra < a.M, a.vecA, va);
+                load8(A + (int64_t)(m0 + ra) * s.lda + k0 + ka, a.K - k0 - ka, m0 + ra < q.M, s.vecA, va);
             } else {
                 ka = tid >> 3, ra = (tid & 7) * 8;
-                load8(A + (int64_t)(k0 + ka) * a.lda + m0 + ra, a.M - m0 - ra, k0 + ka < a.K, a.vecA, va);
+                load8(A + (int64_t)(k0 + ka) * s.lda + m0 + ra, q.M - m0 - ra, k0 + ka < a.K, s.vecA, va);
             }
             // EPI_GATE: rows 0..31 of the tile come from Wg, 32..63 from Wu
             if (BKc) {
                 rb = tid >> 2, kb = (tid & 3) * 8;
                 const int half = EPI == EPI_GATE ? rb / NT : 0, n = n0 + rb - half * NT;
-                load8((const E*)a.B[EPI == EPI_GATE ? half : bi] + (int64_t)n * a.ldb[EPI == EPI_GATE ? half : bi] + k0 + kb, a.K - k0 - kb, n < a.N, a.vecB, vb);
+                const Product& t = EPI == EPI_GATE ? a.p[half] : s;
+                load8((const E*)t.B + (int64_t)n * t.ldb + k0 + kb, a.K - k0 - kb, n < q.N, t.vecB, vb);
             } else {
                 kb = tid >> 3, rb = (tid & 7) * 8;
                 const int half = EPI == EPI_GATE ? rb / NT : 0, n = n0 + rb - half * NT;
-                load8((const E*)a.B[EPI == EPI_GATE ? half : bi] + (int64_t)(k0 + kb) * a.ldb[EPI == EPI_GATE ? half : bi] + n, a.N - n, k0 + kb < a.K, a.vecB, vb);
+                const Product& t = EPI == EPI_GATE ? a.p[half] : s;
+                load8((const E*)t.B + (int64_t)(k0 + kb) * t.ldb + n, q.N - n, k0 + kb < a.K, t.vecB, vb);
             }
             __syncthreads();
 #pragma unroll
@@ -243,22 +283,22 @@ __global__ __launch_bounds__(256) void gemm_any(const Args a) {
                         for (int kk = 0; kk < KS; kk += 16) {
                             const f4 x = *(const f4*)(pb + kk + g * 4), w = *(const f4*)(pa + kk + g * 4);
 #pragma unroll
-                            for (int s = 0; s < 4; ++s) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[s], w[s], acc[i][j], 0, 0, 0);
+                            for (int e = 0; e < 4; ++e) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], w[e], acc[i][j], 0, 0, 0);
                         }
                     }
                 }
         }
     }
     const int r = lane & 15, g = lane >> 4;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int m = m0 + wm * 32 + i * 16 + r;
-        if (m >= a.M) continue;
-        if constexpr (EPI == EPI_GATE)
-            finish<T, EPI>(a, 0, m, n0 + wn * 16 + g * 4, acc[i][0], acc[i][1]);
-        else
-#pragma unroll
-            for (int j = 0; j < 2; ++j) finish<T, EPI>(a, z, m, n0 + wn * 32 + j * 16 + g * 4, acc[i][j], f4{});
+    if constexpr (EPI == EPI_GATE) {
+        const int m[2] = {m0 + wm * 32 + r, m0 + wm * 32 + 16 + r}, n[2] = {n0 + wn * 16 + g * 4, n0 + wn * 16 + g * 4};
+        const f4 c[2] = {acc[0][0], acc[1][0]}, v[2] = {acc[0][1], acc[1][1]};
+        finish<T, EPI, 2>(a, q, m, n, c, v);
+    } else {
+        const int m[4] = {m0 + wm * 32 + r, m0 + wm * 32 + r, m0 + wm * 32 + 16 + r, m0 + wm * 32 + 16 + r};
+        const int n[4] = {n0 + wn * 32 + g * 4, n0 + wn * 32 + 16 + g * 4, n0 + wn * 32 + g * 4, n0 + wn * 32 + 16 + g * 4};
+        const f4 c[4] = {acc[0][0], acc[0][1], acc[1][0], acc[1][1]};
+        finish<T, EPI, 4>(a, q, m, n, c, c);
     }
 }
 
@@ -372,6 +412,31 @@ struct Operand {
     }
 };
 
+// Workgroup b runs on XCD b % 8: each XCD takes a contiguous run of tiles, in groups of 8 rows of tiles, so that its L2 holds the rows of A
+// of a group and a few columns of B
+static __device__ inline int on_its_xcd(int b, int n) {
+    const int each = n / 8, more = n % 8, x = b % 8, l = b / 8;
+    return (x < more ? x * (each + 1) : more * (each + 1) + (x - more) * each) + l;
+}
+struct Place {
+    int z, m0, n0;
+};
+template <int BM, int BN, int HALVES>
+static __device__ inline Place place(const Args& a, int t) {
+    constexpr int GM = 8, NT = BN / HALVES;
+    const bool quarter = BM == 128 && a.quarters;  // (the order of the tiles is then that of the 256 x 256 ones)
+    const int tm = quarter ? 256 : BM, tn = quarter ? 256 / HALVES : NT, corner = quarter ? t % 4 : 0;
+    t = (quarter ? t / 4 : t) + a.first;
+    int z = 0, nm = (a.p[0].M + tm - 1) / tm, nn = (a.p[0].N + tn - 1) / tn;
+    while (z + 1 < a.nprod && t >= nm * nn) {
+        t -= nm * nn;
+        ++z;
+        nm = (a.p[z].M + tm - 1) / tm, nn = (a.p[z].N + tn - 1) / tn;
+    }
+    const int group = t / (GM * nn), gm0 = group * GM, gsize = nm - gm0 < GM ? nm - gm0 : GM;
+    return {z, (gm0 + (t - group * GM * nn) % gsize) * tm + corner % 2 * BM, (t - group * GM * nn) / gsize * tn + corner / 2 * NT};
+}
+
 template <class T, int EPI, bool AK, bool BKc, int BM, int BN, int NWM, int NWN, int OCC>
 __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void gemm_tile(const Args a) {
     constexpr int NW = NWM * NWN, FM = BM / NWM / 16, FN = BN / NWN / 16, HALVES = EPI == EPI_GATE ? 2 : 1;
@@ -381,18 +446,12 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
     constexpr int BUFFERS = 2 * OB::BYTES + 3 * OA::BYTES;  // two of B, then three of A
     __shared__ __attribute__((aligned(1024))) char lds[BUFFERS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % NWM, wn = wave / NWM;
-    const int z = blockIdx.z;
-    // workgroup b runs on XCD b % 8: each XCD takes a contiguous run of tiles, in groups of 8 rows of tiles, so that its L2 holds the
-    // rows of A of a group and a few columns of B
-    const int nm = (a.M + BM - 1) / BM, nn = (a.N + NT - 1) / NT, tiles = nm * nn;
-    int t = (int)blockIdx.x;
-    {
-        const int q = tiles / 8, r = tiles % 8, x = t % 8, l = t / 8;
-        t = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + l;
-    }
-    constexpr int GM = 8;
-    const int group = t / (GM * nn), gm0 = group * GM, gsize = nm - gm0 < GM ? nm - gm0 : GM;
-    const int m0 = (gm0 + (t - group * GM * nn) % gsize) * BM, n0 = (t - group * GM * nn) / gsize * NT;
+    int t = on_its_xcd((int)blockIdx.x, (int)gridDim.x);
+    const int tiles = (int)gridDim.x / a.split, part = t / tiles;
+    const Place at_tile = place<BM, BN, HALVES>(a, t % tiles);
+    const Product& q = a.p[at_tile.z];
+    const int z = at_tile.z, m0 = at_tile.m0, n0 = at_tile.n0;
+    if (m0 >= q.M || n0 >= q.N) return;
 
     f4 acc[FM][FN] = {};
     s8 fa[2][FM], fb[2][FN];
@@ -454,24 +513,28 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
     };
     constexpr int A0 = 2 * OB::BYTES, A1 = A0 + OA::BYTES, A2 = A1 + OA::BYTES;
     // Offsets within a run of steps stay below 2^31: a run of an "R" operand with long rows is shorter than K
-    int64_t most = 1 << 24;
-    if (!AK && (1 << 30) / (128 * a.lda) < most) most = (1 << 30) / (128 * a.lda);
+    int64_t most = 1 << 22;
+    if (!AK && (1 << 30) / (128 * q.lda) < most) most = (1 << 30) / (128 * q.lda);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-        if (!BKc && a.ldb[h] && (1 << 30) / (128 * a.ldb[h]) < most) most = (1 << 30) / (128 * a.ldb[h]);
+        if (!BKc && (h ? HALVES == 2 || a.nseg == 2 : true) && (1 << 30) / (128 * a.p[z + h].ldb) < most) most = (1 << 30) / (128 * a.p[z + h].ldb);
     const int run = (int)most;
-    for (int seg = 0; seg < a.nseg; ++seg)
-        for (int64_t k0 = 0; k0 < a.K; k0 += (int64_t)run * 64) {
+    // this part's steps out of the nseg * ksteps ones
+    const int ksteps = (a.K + 63) / 64, each = (a.nseg * ksteps + a.split - 1) / a.split;
+    for (int seg = 0; seg < a.nseg; ++seg) {
+        const int lo = part * each - seg * ksteps, hi = lo + each;
+        const int64_t kend = hi >= ksteps ? a.K : (int64_t)hi * 64;
+        for (int64_t k0 = lo > 0 ? (int64_t)lo * 64 : 0; k0 < kend; k0 += (int64_t)run * 64) {
             {
-                const int sa = a.nseg > 1 ? seg : z, sb = HALVES == 2 ? 0 : sa;
-                const void* pa[1] = {a.A[sa]};
-                const int64_t la[1] = {a.lda};
-                oa.init(pa, la, m0, a.M, (int)k0, a.K, wave, lane);
-                const void* pb[2] = {a.B[sb], a.B[1]};
-                const int64_t lb[2] = {a.ldb[sb], a.ldb[1]};
-                ob.init(pb, lb, n0, a.N, (int)k0, a.K, wave, lane);
+                const Product& s = a.p[a.nseg > 1 ? seg : z];
+                const void* pa[1] = {s.A};
+                const int64_t la[1] = {s.lda};
+                oa.init(pa, la, m0, q.M, (int)k0, a.K, wave, lane);
+                const void* pb[2] = {s.B, a.p[1].B};
+                const int64_t lb[2] = {s.ldb, a.p[1].ldb};
+                ob.init(pb, lb, n0, q.N, (int)k0, a.K, wave, lane);
             }
-            const int left = (int)((a.K - k0) / 64), full = left < run ? left : run, rest = left < run ? (int)((a.K - k0) % 64) : 0;
+            const int left = (int)((kend - k0) / 64), full = left < run ? left : run, rest = left < run ? (int)((kend - k0) % 64) : 0;
             if (full) {
                 const int last = full - 1;
                 load_a(A0, 0), load_b(0, 0);
@@ -509,30 +572,73 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             }
         }
+    }
+    if (a.split > 1) {
+        f4* to = (f4*)a.part + (((int64_t)(t % tiles) * a.split + part) * NW + wave) * FM * FN * 64 + lane;
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) to[(i * FN + j) * 64] = acc[i][j];
+        return;
+    }
     // epilogue: 32 rows of a wavefront at a time through LDS, so that the code of finish() stands in a loop and a row's lanes store side by
-    // side.  (The rows are four floats longer than they need to be: 8 lanes that write 16 bytes of 8 rows touch every bank once.)
-    constexpr int COLS = BN / NWN, LDC = COLS + 4, CT = COLS / HALVES;
-    static_assert(NW * 32 * LDC * 4 <= BUFFERS, "epilogue");
+    // side, up to four stores a turn.  (The rows are four floats longer than they need to be: 8 lanes that write 16 bytes of 8 rows touch every
+    // bank once.)
+    constexpr int COLS = BN / NWN, LDC = COLS + 4, CT = COLS / HALVES, TURN = 32 * CT / 4 < 256 ? 32 * CT / 4 / 64 : 4;
+    static_assert(NW * 32 * LDC * 4 <= BUFFERS && 32 * CT / 4 % (64 * TURN) == 0, "epilogue");
     float* mine = (float*)lds + wave * 32 * LDC;
-#pragma unroll
+#pragma unroll 1
     for (int p = 0; p < FM / 2; ++p) {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (m0 + wm * (BM / NWM) + p * 32 >= q.M) break;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < FM; ++i)
+            if (i / 2 == p)
 #pragma unroll
-            for (int j = 0; j < FN; ++j) *(f4*)(mine + (i * 16 + (lane & 15)) * LDC + j * 16 + (lane >> 4) * 4) = acc[2 * p + i][j];
+                for (int j = 0; j < FN; ++j) *(f4*)(mine + (i % 2 * 16 + (lane & 15)) * LDC + j * 16 + (lane >> 4) * 4) = acc[i][j];
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll 1
-        for (int e = lane; e < 32 * CT / 4; e += 64) {
-            const int row = e / (CT / 4), col = e % (CT / 4) * 4, m = m0 + wm * (BM / NWM) + p * 32 + row;
-            if (m >= a.M) break;
-            const f4 c = *(const f4*)(mine + row * LDC + col);
-            if constexpr (EPI == EPI_GATE)
-                finish<T, EPI>(a, 0, m, n0 + wn * CT + col, c, *(const f4*)(mine + row * LDC + CT + col));
-            else
-                finish<T, EPI>(a, z, m, n0 + wn * CT + col, c, f4{});
+        for (int e0 = lane; e0 < 32 * CT / 4; e0 += 64 * TURN) {
+            int m[TURN], n[TURN];
+            f4 c[TURN], v[TURN];
+#pragma unroll
+            for (int i = 0; i < TURN; ++i) {
+                const int row = (e0 + 64 * i) / (CT / 4), col = (e0 + 64 * i) % (CT / 4) * 4;
+                m[i] = m0 + wm * (BM / NWM) + p * 32 + row;
+                n[i] = n0 + wn * CT + col;
+                c[i] = *(const f4*)(mine + row * LDC + col);
+                v[i] = EPI == EPI_GATE ? *(const f4*)(mine + row * LDC + CT + col) : f4{};
+            }
+            finish<T, EPI, TURN>(a, q, m, n, c, v);
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
+}
+
+// Adds up the parts of K of a tile, in their order, and does what the tile kernel would have done with the sums.  One wavefront per 16 rows of
+// a wavefront's tile; the parts lie as the lanes held them, so that every access is one contiguous 1 KB.
+template <class T, int EPI, int BM, int BN, int NWM, int NWN>
+__global__ __launch_bounds__(64 * NWM * NWN) void join_parts(const Args a) {
+    constexpr int NW = NWM * NWN, FM = BM / NWM / 16, FN = BN / NWN / 16, HALVES = EPI == EPI_GATE ? 2 : 1, NT = BN / HALVES;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % NWM, wn = wave / NWM, i = blockIdx.y;
+    const Place at = place<BM, BN, HALVES>(a, (int)blockIdx.x);
+    const Product& q = a.p[at.z];
+    const f4* from = (const f4*)a.part + (((int64_t)blockIdx.x * a.split) * NW + wave) * FM * FN * 64 + i * FN * 64 + lane;
+    f4 sum[FN] = {};
+#pragma unroll 4
+    for (int s = 0; s < a.split; ++s)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) sum[j] += from[((int64_t)s * NW * FM * FN + j) * 64];
+    constexpr int N = FN / HALVES;
+    int m[N], n[N];
+    f4 c[N], v[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        m[j] = at.m0 + wm * (BM / NWM) + i * 16 + (lane & 15);
+        n[j] = at.n0 + wn * (NT / NWN) + j * 16 + (lane >> 4) * 4;
+        c[j] = sum[j];
+        v[j] = sum[j + FN - N];
+    }
+    finish<T, EPI, N>(a, q, m, n, c, v);
 }
 
 }  // namespace gated
