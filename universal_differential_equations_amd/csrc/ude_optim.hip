@@ -36,8 +36,8 @@ struct DBF16 {
 };
 
 constexpr int ADAM_NT = 44, NORM_NT = 160;
-constexpr int64_t ADAM_CHUNK = 4096;   // elements of one workgroup (a multiple of UDE_ADAMW_BLOCK)
-constexpr int64_t NORM_CHUNK = 16384;
+constexpr int64_t ADAM_CHUNK = 4096;   // elements of one workgroup: 16 a thread
+constexpr int64_t NORM_CHUNK = 4096;
 constexpr int NORM_BLOCKS = 2048;
 constexpr int64_t MOST_CHUNKS = (int64_t)1 << 23;                   // of one launch: 256 threads each, fewer than 2^32
 constexpr int64_t MOST_ELEMENTS = MOST_CHUNKS * ADAM_CHUNK;         // of one tensor
@@ -105,110 +105,251 @@ __device__ inline float root(float x) { return sqrtf(x); }
 template <>
 __device__ inline double root(double x) { return sqrt(x); }
 
+// N consecutive elements as one or a few 16-byte (or one shorter) accesses; p is aligned to them
+template <int N, class E>
+__device__ inline void get(const E* p, E* o) {
+    constexpr int V = 16 / sizeof(E) < N ? 16 / sizeof(E) : N;
+    typedef E T __attribute__((ext_vector_type(V)));
+#pragma unroll
+    for (int i = 0; i < N / V; ++i) {
+        const T x = ((const T*)p)[i];
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[i * V + j] = x[j];
+    }
+}
+template <int N, class E>
+__device__ inline void put(E* p, const E* o) {
+    constexpr int V = 16 / sizeof(E) < N ? 16 / sizeof(E) : N;
+    typedef E T __attribute__((ext_vector_type(V)));
+#pragma unroll
+    for (int i = 0; i < N / V; ++i) {
+        T x;
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[j] = o[i * V + j];
+        ((T*)p)[i] = x;
+    }
+}
+template <int N, class E>
+__host__ __device__ inline bool fits(const E* p) {
+    return (uintptr_t)p % (N * sizeof(E) < 16 ? N * sizeof(E) : 16) == 0;
+}
+
+// Bound by memory: 28 bytes an element with 16-bit parameters and 32-bit copies.  A thread has 16 elements of a chunk, four at a time side by
+// side where the tensor's pointers allow it, and asks for all of them before it uses the first: a small tensor costs one trip to memory.
 template <class P, class G>
 __global__ __launch_bounds__(256) void adamw32_kernel(const AdamArgs a) {
     typedef typename P::W W;
-    W s, rate, rc2;
-    if (!step_factors<W>(a, s, rate, rc2)) return;
+    typedef typename P::E PE;
+    typedef typename G::E GE;
     const int k = tensor_of(a, (int)blockIdx.x);
     const AdamTensor& t = a.t[k];
     const int64_t at = (int64_t)((int)blockIdx.x - a.first[k]) * ADAM_CHUNK;
-    const W keep = (W)(1 - a.eta * t.wd), b1 = (W)a.b1, d1 = (W)(1 - a.b1), b2 = (W)a.b2, d2 = (W)(1 - a.b2), eps = (W)a.eps;
     const int64_t end = t.n < at + ADAM_CHUNK ? t.n : at + ADAM_CHUNK;
-    typename P::E* p = (typename P::E*)t.p;
-    const typename G::E* g = (const typename G::E*)t.g;
-    W *m = (W*)t.m, *v = (W*)t.v;
-    for (int64_t i = at + threadIdx.x; i < end; i += 256) {
-        const W gr = (W)g[i] * s;
-        const W mi = b1 * m[i] + d1 * gr, vi = b2 * v[i] + d2 * gr * gr;
-        m[i] = mi;
-        v[i] = vi;
-        W w = t.master ? (W)t.master[i] : (W)p[i];
-        w = w * keep - rate * mi / (root<W>(vi * rc2) + eps);
-        if (t.master) t.master[i] = (float)w;
-        p[i] = (typename P::E)w;
+    PE* const p = (PE*)t.p;
+    const GE* const g = (const GE*)t.g;
+    W *const m = (W*)t.m, *const v = (W*)t.v;
+    float* const master = t.master;
+    PE pp[16];
+    GE gg[16];
+    W mm[16], vv[16];
+    float ww[16];
+    const bool four = end == at + ADAM_CHUNK && fits<4>(p) && fits<4>(g) && fits<4>(m) && fits<4>(v) && fits<4>(master);
+    if (four) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t i = at + j * 1024 + threadIdx.x * 4;
+            get<4>(g + i, gg + 4 * j);
+            get<4>(m + i, mm + 4 * j);
+            get<4>(v + i, vv + 4 * j);
+            if (master)
+                get<4>(master + i, ww + 4 * j);
+            else
+                get<4>(p + i, pp + 4 * j);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int64_t i = at + j * 256 + threadIdx.x;
+            const bool in = i < end;
+            gg[j] = in ? g[i] : (GE)0;
+            mm[j] = in ? m[i] : (W)0;
+            vv[j] = in ? v[i] : (W)0;
+            if (master)
+                ww[j] = in ? master[i] : 0.f;
+            else
+                pp[j] = in ? p[i] : (PE)0;
+        }
+    }
+    W s, rate, rc2;
+    if (!step_factors<W>(a, s, rate, rc2)) return;
+    const W keep = (W)(1 - a.eta * t.wd), b1 = (W)a.b1, d1 = (W)(1 - a.b1), b2 = (W)a.b2, d2 = (W)(1 - a.b2), eps = (W)a.eps;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const W gr = (W)gg[j] * s;
+        mm[j] = b1 * mm[j] + d1 * gr;
+        vv[j] = b2 * vv[j] + d2 * gr * gr;
+        W w = master ? (W)ww[j] : (W)pp[j];
+        w = w * keep - rate * mm[j] / (root<W>(vv[j] * rc2) + eps);
+        ww[j] = (float)w;
+        pp[j] = (PE)w;
+    }
+    if (four) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t i = at + j * 1024 + threadIdx.x * 4;
+            put<4>(m + i, mm + 4 * j);
+            put<4>(v + i, vv + 4 * j);
+            put<4>(p + i, pp + 4 * j);
+            if (master) put<4>(master + i, ww + 4 * j);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int64_t i = at + j * 256 + threadIdx.x;
+            if (i < end) {
+                m[i] = mm[j];
+                v[i] = vv[j];
+                p[i] = pp[j];
+                if (master) master[i] = ww[j];
+            }
+        }
     }
 }
 
-// Codes of the 8-bit moments.  A code is decided in Float64: a Float32 root gives the candidate, the borders (q - 1/2)^2, (q + 1/2)^2 (and
-// their squares) are whole numbers plus a power of two, exact in Float64, and move it by one where the root was on the wrong side.
-__device__ inline int code_m(double y) {  // y = 127^2 |m| / a
-    int q = (int)rintf(sqrtf((float)y));
-    const double lo = (double)(q * q - q) + 0.25, hi = (double)(q * q + q) + 0.25;
-    if (q > 0 && y < lo) --q;
-    if (y >= hi) ++q;
-    return q > 127 ? 127 : q;
+// Codes of the 8-bit moments, decided in Float64.  With y = 127^2 |m| / a (255^4 v / c) the code is the q with (q - 1/2)^2 <= y < (q + 1/2)^2
+// (the same squared).  A Float32 root, less what it may be too large by, gives q or q - 1; the border between the two is a whole number
+// plus 1/4 below 2^17 (exact in Float32; its square has at most 38 bits) and is compared with y in Float64.
+__device__ inline int code_m(double y) {
+    const int q = (int)(__builtin_amdgcn_sqrtf((float)y) + 0.4999f);  // roots up to 127, a few 2^-24 of them off
+    const float border = (float)(q * q + q) + 0.25f;
+    const int r = y >= (double)border ? q + 1 : q;
+    return r > 127 ? 127 : r;
 }
-__device__ inline int code_v(double y) {  // y = 255^4 v / c
-    int q = (int)rintf(sqrtf(sqrtf((float)y)));
-    const double lo = (double)(q * q - q) + 0.25, hi = (double)(q * q + q) + 0.25;
-    if (q > 0 && y < lo * lo) --q;
-    if (y >= hi * hi) ++q;
-    q = q > 255 ? 255 : q;
-    return q == 0 && y > 0 ? 1 : q;
+__device__ inline int code_v(double y) {
+    const int q = (int)(__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)y)) + 0.499f);
+    const double border = (double)((float)(q * q + q) + 0.25f);
+    const int r = y >= border * border ? q + 1 : q;
+    return r > 255 ? 255 : r == 0 && y > 0 ? 1 : r;
 }
-__device__ inline double value_m(int q, double a) { return a * ((double)(q * (q < 0 ? -q : q)) * (1.0 / 16129.0)); }
-__device__ inline double value_v(int r, double c) { return c * ((double)(unsigned)(r * r) * (double)(unsigned)(r * r) * (1.0 / 4228250625.0)); }
+// what a code stands for, over the scale: signed squares of up to 14 bits, fourth powers of up to 32
+__device__ inline double m_part(int q) { return (double)(q * (q < 0 ? -q : q)); }
+__device__ inline double v_part(int r) { return (double)((unsigned)(r * r) * (unsigned)(r * r)); }
+constexpr double M_UNIT = 1.0 / 16129.0, V_UNIT = 1.0 / 4228250625.0;
 
-// 16 lanes hold one block of 256 elements, 16 consecutive ones each: a code row is one 16-byte load, the two maxima are four exchanges
+// the largest of 16 lanes' values, as whole numbers (that is the order of floats >= 0, and above them infinity and NaN), by rotations in a row of 16
+__device__ inline int row_max(int x) {
+    x = max(x, __builtin_amdgcn_mov_dpp(x, 0x128, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_mov_dpp(x, 0x124, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_mov_dpp(x, 0x122, 0xf, 0xf, false));
+    return max(x, __builtin_amdgcn_mov_dpp(x, 0x121, 0xf, 0xf, false));
+}
+
+// 16 lanes hold one block of 256 elements, 8 consecutive ones of each half, so that the 16-byte accesses of 16-bit parameters lie side by
+// side.  About as much arithmetic (60 to 70 instructions an element, a third of them Float64) as memory time.
 template <class P, class G>
 __global__ __launch_bounds__(256) void adamw8_kernel(const AdamArgs a) {
+    typedef typename P::E PE;
+    typedef typename G::E GE;
+    const int k = tensor_of(a, (int)blockIdx.x);
+    const AdamTensor& t = a.t[k];
+    const int64_t block = (int64_t)((int)blockIdx.x - a.first[k]) * (ADAM_CHUNK / UDE_ADAMW_BLOCK) + threadIdx.x / 16;
+    const int64_t at = block * UDE_ADAMW_BLOCK + (threadIdx.x & 15) * 8;
+    const bool any = block * UDE_ADAMW_BLOCK < t.n;
+    PE* const p = (PE*)t.p + at;
+    const GE* const g = (const GE*)t.g + at;
+    int8_t* const mq = (int8_t*)t.m + at;
+    uint8_t* const vq = (uint8_t*)t.v + at;
+    float* const master = t.master ? t.master + at : nullptr;
+    PE pp[16];
+    GE gg[16];
+    int8_t mm[16];
+    uint8_t vv[16];
+    float ww[16];
+    // (the same for a whole block: its elements lie behind one another)
+    const bool eight = (block + 1) * UDE_ADAMW_BLOCK <= t.n && fits<8>(p) && fits<8>(g) && fits<8>(mq) && fits<8>(vq) && fits<8>(master);
+    if (eight) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            get<8>(g + 128 * h, gg + 8 * h);
+            get<8>(mq + 128 * h, mm + 8 * h);
+            get<8>(vq + 128 * h, vv + 8 * h);
+            if (master)
+                get<8>(master + 128 * h, ww + 8 * h);
+            else
+                get<8>(p + 128 * h, pp + 8 * h);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int e = i / 8 * 128 + i % 8;
+            const bool in = at + e < t.n;
+            gg[i] = in ? g[e] : (GE)0;
+            mm[i] = in ? mq[e] : (int8_t)0;
+            vv[i] = in ? vq[e] : (uint8_t)0;
+            if (master)
+                ww[i] = in ? master[e] : 0.f;
+            else
+                pp[i] = in ? p[e] : (PE)0;
+        }
+    }
+    const double sa = any ? (double)t.ms[block] : 0, sc = any ? (double)t.vs[block] : 0;
     float s, rate, rc2;
     if (!step_factors<float>(a, s, rate, rc2)) return;
     const double factor = a.clip ? a.clip[1] : 1.0;
-    const int k = tensor_of(a, (int)blockIdx.x);
-    const AdamTensor& t = a.t[k];
-    const int64_t at = (int64_t)((int)blockIdx.x - a.first[k]) * ADAM_CHUNK + threadIdx.x * 16;
-    const float keep = (float)(1 - a.eta * t.wd), eps = (float)a.eps;
-    const int64_t left = t.n - at;
-    const int n = left < 0 ? 0 : left > 16 ? 16 : (int)left;
-    const int64_t block = at / UDE_ADAMW_BLOCK;
-    typename P::E* p = (typename P::E*)t.p + at;
-    const typename G::E* g = (const typename G::E*)t.g + at;
-    int8_t* mq = (int8_t*)t.m + at;
-    uint8_t* vq = (uint8_t*)t.v + at;
-    float* master = t.master ? t.master + at : nullptr;
-    double am = 0, av = 0;
-    float bad = 0;
+    const double d1 = 1 - a.b1, d2 = 1 - a.b2;
     double m[16], v[16];
-    const bool any = block * UDE_ADAMW_BLOCK < t.n;
-    const double sa = any ? (double)t.ms[block] : 0, sc = any ? (double)t.vs[block] : 0;
+    int am = 0, av = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {  // (elements behind the end: codes and gradients of zero)
+        // (in the order of the formula: constants multiplied beforehand would round otherwise, and a largest element whose gradient comes
+        // again lies half way between two scales more often than chance has it)
+        const double x = (double)(float)gg[i] * factor;
+        m[i] = a.b1 * (m_part(mm[i]) * M_UNIT * sa) + d1 * x;
+        v[i] = a.b2 * (v_part(vv[i]) * V_UNIT * sc) + d2 * (x * x);
+        am = max(am, __float_as_int(fabsf((float)m[i])));
+        av = max(av, __float_as_int(fabsf((float)v[i])));
+    }
+    am = row_max(am);
+    av = row_max(av);
+    // (a gradient that is not finite makes the moments of its block NaN)
+    const bool bad = am >= 0x7f800000 || av >= 0x7f800000;
+    const float fa = bad ? __builtin_nanf("") : __int_as_float(am), fc = bad ? __builtin_nanf("") : __int_as_float(av);
+    const double ia = fa > 0 ? 16129.0 / (double)fa : 0, ic = fc > 0 ? 4228250625.0 / (double)fc : 0;
+    const float keep = (float)(1 - a.eta * t.wd), eps = (float)a.eps;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        m[i] = v[i] = 0;
-        if (i < n) {
-            const double gr = (double)(float)g[i] * factor;
-            m[i] = a.b1 * value_m(mq[i], sa) + (1 - a.b1) * gr;
-            v[i] = a.b2 * value_v(vq[i], sc) + (1 - a.b2) * gr * gr;
-            bad += (float)(m[i] - m[i]) + (float)(v[i] - v[i]);
-            am = fmax(am, fabs(m[i]));
-            av = fmax(av, v[i]);
-        }
+        const int q = code_m(fabs(m[i]) * ia);
+        mm[i] = (int8_t)(m[i] < 0 ? -q : q);
+        vv[i] = (uint8_t)code_v(v[i] * ic);
+        float w = master ? ww[i] : (float)pp[i];
+        w = w * keep - rate * (float)m[i] / (sqrtf((float)v[i] * rc2) + eps);
+        ww[i] = w;
+        pp[i] = (PE)w;
     }
-#pragma unroll
-    for (int d = 1; d < 16; d *= 2) {
-        am = fmax(am, __shfl_xor(am, d, 64));
-        av = fmax(av, __shfl_xor(av, d, 64));
-        bad += __shfl_xor(bad, d, 64);
-    }
-    // (a gradient that is not finite makes the moments of its block NaN: they are then read as such)
-    const float fa = (float)am + bad, fc = (float)av + bad;
     if (any && (threadIdx.x & 15) == 0) {
         t.ms[block] = fa;
         t.vs[block] = fc;
     }
-    const double ia = fa > 0 ? 16129.0 / (double)fa : 0, ic = fc > 0 ? 4228250625.0 / (double)fc : 0;
+    if (eight) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-        if (i < n) {
-            const int q = code_m(fabs(m[i]) * ia);
-            mq[i] = (int8_t)(m[i] < 0 ? -q : q);
-            vq[i] = (uint8_t)code_v(v[i] * ic);
-            float w = master ? master[i] : (float)p[i];
-            w = w * keep - rate * (float)m[i] / (sqrtf((float)v[i] * rc2) + eps);
-            if (master) master[i] = w;
-            p[i] = (typename P::E)w;
+        for (int h = 0; h < 2; ++h) {
+            put<8>(mq + 128 * h, mm + 8 * h);
+            put<8>(vq + 128 * h, vv + 8 * h);
+            put<8>(p + 128 * h, pp + 8 * h);
+            if (master) put<8>(master + 128 * h, ww + 8 * h);
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int e = i / 8 * 128 + i % 8;
+            if (at + e < t.n) {
+                mq[e] = mm[i];
+                vq[e] = vv[i];
+                p[e] = pp[i];
+                if (master) master[e] = ww[i];
+            }
+        }
+    }
 }
 
 struct MomentTensor {
@@ -230,9 +371,26 @@ __global__ __launch_bounds__(256) void moments_kernel(const MomentArgs a) {
     const MomentTensor& t = a.t[k];
     const int64_t at = (int64_t)((int)blockIdx.x - a.first[k]) * ADAM_CHUNK;
     const int64_t end = t.n < at + ADAM_CHUNK ? t.n : at + ADAM_CHUNK;
-    for (int64_t i = at + threadIdx.x; i < end; i += 256) {
-        t.mo[i] = (float)value_m(t.m[i], (double)t.ms[i / UDE_ADAMW_BLOCK]);
-        t.vo[i] = (float)value_v(t.v[i], (double)t.vs[i / UDE_ADAMW_BLOCK]);
+    if (end == at + ADAM_CHUNK && fits<8>(t.m) && fits<8>(t.v) && fits<8>(t.mo) && fits<8>(t.vo)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t i = at + h * 2048 + threadIdx.x * 8;
+            const double sa = (double)t.ms[i / UDE_ADAMW_BLOCK], sc = (double)t.vs[i / UDE_ADAMW_BLOCK];
+            int8_t m[8];
+            uint8_t v[8];
+            float mo[8], vo[8];
+            get<8>(t.m + i, m);
+            get<8>(t.v + i, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mo[j] = (float)(m_part(m[j]) * M_UNIT * sa), vo[j] = (float)(v_part(v[j]) * V_UNIT * sc);
+            put<8>(t.mo + i, mo);
+            put<8>(t.vo + i, vo);
+        }
+    } else {
+        for (int64_t i = at + threadIdx.x; i < end; i += 256) {
+            t.mo[i] = (float)(m_part(t.m[i]) * M_UNIT * (double)t.ms[i / UDE_ADAMW_BLOCK]);
+            t.vo[i] = (float)(v_part(t.v[i]) * V_UNIT * (double)t.vs[i / UDE_ADAMW_BLOCK]);
+        }
     }
 }
 
@@ -257,19 +415,33 @@ __device__ inline double block_sum(double x) {
 
 template <class G>
 __global__ __launch_bounds__(256) void norm_part_kernel(const NormArgs a) {
-    double sum = 0;
+    typedef typename G::E E;
+    constexpr int V = 16 / sizeof(E);
+    double sum[4] = {};
     for (int c = (int)blockIdx.x; c < a.chunks; c += (int)gridDim.x) {
         const int k = tensor_of(a, c);
         const int64_t at = (int64_t)(c - a.first[k]) * NORM_CHUNK;
         const int64_t end = a.n[k] < at + NORM_CHUNK ? a.n[k] : at + NORM_CHUNK;
-        const typename G::E* g = (const typename G::E*)a.g[k];
-        for (int64_t i = at + threadIdx.x; i < end; i += 256) {
-            const double x = (double)(typename G::W)g[i];
-            sum += x * x;
+        const E* g = (const E*)a.g[k];
+        E x[16];
+        if (end == at + NORM_CHUNK && fits<V>(g)) {
+#pragma unroll
+            for (int j = 0; j < 16 / V; ++j) get<V>(g + at + j * 256 * V + threadIdx.x * V, x + j * V);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int64_t i = at + j * 256 + threadIdx.x;
+                x[j] = i < end ? g[i] : (E)0;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const double y = (double)(typename G::W)x[j];
+            sum[j % 4] = fma(y, y, sum[j % 4]);
         }
     }
-    sum = block_sum(sum);
-    if (threadIdx.x == 0) a.part[blockIdx.x] = sum;
+    const double all = block_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
+    if (threadIdx.x == 0) a.part[blockIdx.x] = all;
 }
 
 __global__ __launch_bounds__(256) void norm_join_kernel(const double* part, int n, double max_norm, double* out) {
