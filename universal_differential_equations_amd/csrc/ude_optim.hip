@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "ude_ctx.h"
 
@@ -36,11 +37,13 @@ struct DBF16 {
 };
 
 constexpr int ADAM_NT = 44, NORM_NT = 160;
-constexpr int64_t ADAM_CHUNK = 4096;   // elements of one workgroup: 16 a thread
+constexpr int64_t ADAM_CHUNK = 4096;    // elements of one workgroup that writes out 8-bit moments' values: 16 a thread
+constexpr int64_t ADAM8_CHUNK = 4096;   // with 8-bit moments: 16 a thread
+constexpr int64_t ADAM32_CHUNK = 1024;  // with 32-bit moments: 4 a thread
 constexpr int64_t NORM_CHUNK = 4096;
 constexpr int NORM_BLOCKS = 2048;
 constexpr int64_t MOST_CHUNKS = (int64_t)1 << 23;                   // of one launch: 256 threads each, fewer than 2^32
-constexpr int64_t MOST_ELEMENTS = MOST_CHUNKS * ADAM_CHUNK;         // of one tensor
+constexpr int64_t MOST_ELEMENTS = MOST_CHUNKS * ADAM32_CHUNK;       // of one tensor
 
 struct AdamTensor {
     void* p;
@@ -134,8 +137,8 @@ __host__ __device__ inline bool fits(const E* p) {
     return (uintptr_t)p % (N * sizeof(E) < 16 ? N * sizeof(E) : 16) == 0;
 }
 
-// Bound by memory: 28 bytes an element with 16-bit parameters and 32-bit copies.  A thread has 16 elements of a chunk, four at a time side by
-// side where the tensor's pointers allow it, and asks for all of them before it uses the first: a small tensor costs one trip to memory.
+// Bound by memory: 28 bytes an element with 16-bit parameters and 32-bit copies.  A thread has 4 elements, side by side where the tensor's
+// pointers allow it, and asks for all of them before it uses the first.
 template <class P, class G>
 __global__ __launch_bounds__(256) void adamw32_kernel(const AdamArgs a) {
     typedef typename P::W W;
@@ -143,34 +146,30 @@ __global__ __launch_bounds__(256) void adamw32_kernel(const AdamArgs a) {
     typedef typename G::E GE;
     const int k = tensor_of(a, (int)blockIdx.x);
     const AdamTensor& t = a.t[k];
-    const int64_t at = (int64_t)((int)blockIdx.x - a.first[k]) * ADAM_CHUNK;
-    const int64_t end = t.n < at + ADAM_CHUNK ? t.n : at + ADAM_CHUNK;
+    const int64_t at = (int64_t)((int)blockIdx.x - a.first[k]) * ADAM32_CHUNK;
     PE* const p = (PE*)t.p;
     const GE* const g = (const GE*)t.g;
     W *const m = (W*)t.m, *const v = (W*)t.v;
     float* const master = t.master;
-    PE pp[16];
-    GE gg[16];
-    W mm[16], vv[16];
-    float ww[16];
-    const bool four = end == at + ADAM_CHUNK && fits<4>(p) && fits<4>(g) && fits<4>(m) && fits<4>(v) && fits<4>(master);
+    PE pp[4];
+    GE gg[4];
+    W mm[4], vv[4];
+    float ww[4];
+    const bool four = at + ADAM32_CHUNK <= t.n && fits<4>(p) && fits<4>(g) && fits<4>(m) && fits<4>(v) && fits<4>(master);
+    const int64_t i4 = at + threadIdx.x * 4;
     if (four) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t i = at + j * 1024 + threadIdx.x * 4;
-            get<4>(g + i, gg + 4 * j);
-            get<4>(m + i, mm + 4 * j);
-            get<4>(v + i, vv + 4 * j);
-            if (master)
-                get<4>(master + i, ww + 4 * j);
-            else
-                get<4>(p + i, pp + 4 * j);
-        }
+        get<4>(g + i4, gg);
+        get<4>(m + i4, mm);
+        get<4>(v + i4, vv);
+        if (master)
+            get<4>(master + i4, ww);
+        else
+            get<4>(p + i4, pp);
     } else {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
+        for (int j = 0; j < 4; ++j) {
             const int64_t i = at + j * 256 + threadIdx.x;
-            const bool in = i < end;
+            const bool in = i < t.n;
             gg[j] = in ? g[i] : (GE)0;
             mm[j] = in ? m[i] : (W)0;
             vv[j] = in ? v[i] : (W)0;
@@ -184,7 +183,7 @@ __global__ __launch_bounds__(256) void adamw32_kernel(const AdamArgs a) {
     if (!step_factors<W>(a, s, rate, rc2)) return;
     const W keep = (W)(1 - a.eta * t.wd), b1 = (W)a.b1, d1 = (W)(1 - a.b1), b2 = (W)a.b2, d2 = (W)(1 - a.b2), eps = (W)a.eps;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
+    for (int j = 0; j < 4; ++j) {
         const W gr = (W)gg[j] * s;
         mm[j] = b1 * mm[j] + d1 * gr;
         vv[j] = b2 * vv[j] + d2 * gr * gr;
@@ -194,19 +193,15 @@ __global__ __launch_bounds__(256) void adamw32_kernel(const AdamArgs a) {
         pp[j] = (PE)w;
     }
     if (four) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t i = at + j * 1024 + threadIdx.x * 4;
-            put<4>(m + i, mm + 4 * j);
-            put<4>(v + i, vv + 4 * j);
-            put<4>(p + i, pp + 4 * j);
-            if (master) put<4>(master + i, ww + 4 * j);
-        }
+        put<4>(m + i4, mm);
+        put<4>(v + i4, vv);
+        put<4>(p + i4, pp);
+        if (master) put<4>(master + i4, ww);
     } else {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
+        for (int j = 0; j < 4; ++j) {
             const int64_t i = at + j * 256 + threadIdx.x;
-            if (i < end) {
+            if (i < t.n) {
                 m[i] = mm[j];
                 v[i] = vv[j];
                 p[i] = pp[j];
@@ -252,7 +247,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const AdamArgs a) {
     typedef typename G::E GE;
     const int k = tensor_of(a, (int)blockIdx.x);
     const AdamTensor& t = a.t[k];
-    const int64_t block = (int64_t)((int)blockIdx.x - a.first[k]) * (ADAM_CHUNK / UDE_ADAMW_BLOCK) + threadIdx.x / 16;
+    const int64_t block = (int64_t)((int)blockIdx.x - a.first[k]) * (ADAM8_CHUNK / UDE_ADAMW_BLOCK) + threadIdx.x / 16;
     const int64_t at = block * UDE_ADAMW_BLOCK + (threadIdx.x & 15) * 8;
     const bool any = block * UDE_ADAMW_BLOCK < t.n;
     PE* const p = (PE*)t.p + at;
@@ -534,7 +529,7 @@ extern "C" int ude_adamw_step_dev(ude_ctx* c, const ude_adamw_opts* o, int64_t n
     a.c1 = 1 - pow(o->beta1, (double)o->step), a.c2 = 1 - pow(o->beta2, (double)o->step);
     a.step_dev = o->step_dev, a.clip = o->clip, a.skip = o->skip_nonfinite;
     return in_launches(
-        nt, ADAM_NT, ADAM_CHUNK, a.first, [&](int64_t i) { return ts[i].n; },
+        nt, ADAM_NT, o->state_bits == 8 ? ADAM8_CHUNK : ADAM32_CHUNK, a.first, [&](int64_t i) { return ts[i].n; },
         [&](int slot, int64_t i) {
             const ude_adamw_tensor& t = ts[i];
             a.t[slot] = {t.param, t.grad, t.master, t.m, t.v, t.m_scale, t.v_scale, t.n, t.weight_decay};

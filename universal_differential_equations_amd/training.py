@@ -12,10 +12,12 @@ scenario_1's stored losses); `bfgs` is a plain inverse-Hessian BFGS with Armijo 
 examples that do not compare with an artifact).
 """
 import ctypes as C
+from array import array
 
 import numpy as np
 
 from . import _lib
+from .sciml import Engine
 
 
 def _xp(x):
@@ -61,15 +63,14 @@ def _device_list(what, tensors):
     name = str(dt)[6:]
     if name not in _lib.DTYPE_CODE:
         raise ValueError("%s: tensor 0 is %s: float64, float32, float16 and bfloat16 are supported" % (what, dt))
-    for i, t in enumerate(tensors):
-        if t.device != dev or t.dtype != dt:
-            raise ValueError("%s: tensor %d is %s on %s, tensor 0 %s on %s" % (what, i, t.dtype, t.device, dt, dev))
+    if {t.dtype for t in tensors} != {dt} or {t.get_device() for t in tensors} != {dev.index}:
+        i = next(i for i, t in enumerate(tensors) if t.device != dev or t.dtype != dt)
+        raise ValueError("%s: tensor %d is %s on %s, tensor 0 %s on %s" % (what, i, tensors[i].dtype, tensors[i].device, dt, dev))
     return dev, name
 
 
 def _bound_engine(dev):
     import torch
-    from .sciml import Engine
     eng = Engine.get(dev.index)
     eng.set_stream(torch.cuda.current_stream(dev).cuda_stream)
     return eng
@@ -83,12 +84,14 @@ def grad_norm(grads, max_norm=0.0):
     grads = [g if g.is_contiguous() else g.contiguous() for g in grads if g is not None]
     dev, name = _device_list("grad_norm", grads)
     n = len(grads)
-    ptrs, sizes = (C.c_void_p * n)(*[g.data_ptr() for g in grads]), (C.c_int64 * n)(*[g.numel() for g in grads])
+    ptrs, sizes = array("Q", [g.data_ptr() for g in grads]), array("q", [g.numel() for g in grads])
+    ptrs_at, sizes_at = ptrs.buffer_info()[0], sizes.buffer_info()[0]
     eng = _bound_engine(dev)
     need = C.c_int64(0)
-    eng.check(eng.L.ude_grad_norm_workspace(n, sizes, C.byref(need)))
+    eng.check(eng.L.ude_grad_norm_workspace(n, sizes_at, C.byref(need)))
     buf = torch.empty(2 + need.value // 8, dtype=torch.float64, device=dev)   # [norm, factor] and the partial sums behind them
-    eng.check(eng.L.ude_grad_norm_dev(eng.h, _lib.DTYPE_CODE[name], n, ptrs, sizes, float(max_norm), buf.data_ptr(), buf.data_ptr() + 16, need.value))
+    at = buf.data_ptr()
+    eng.check(eng.L.ude_grad_norm_dev(eng.h, _lib.DTYPE_CODE[name], n, ptrs_at, sizes_at, float(max_norm), at, at + 16, need.value))
     return buf[:2]
 
 
@@ -133,6 +136,7 @@ class AdamW:
             raise ValueError("AdamW: state of %d tensors for %d parameters" % (len(state), n))
         self._state = [self._make_state(i, master, None if state is None else state[i]) for i in range(n)]
         self._table = (_lib.AdamwTensor * n)()
+        self._columns = np.frombuffer(self._table, dtype=np.int64).reshape(n, -1)   # the same memory; column 0: param, 1: grad, 7: n
         self._live = [0] * n
         for i, p in enumerate(self.params):
             s, t = self._state[i], self._table[i]
@@ -140,6 +144,7 @@ class AdamW:
             t.m_scale, t.v_scale = (s[k].data_ptr() if k in s else None for k in ("m_scale", "v_scale"))
             t.param, t.n, t.weight_decay = p.data_ptr(), p.numel(), decay[i]
             self._live[i] = p.numel()
+        self._at = [p.data_ptr() for p in self.params]
         self._opts = _lib.AdamwOpts(param_dtype=_lib.DTYPE_CODE[self.dtype], state_bits=bits)
 
     def _make_state(self, i, master, given):
@@ -176,25 +181,27 @@ class AdamW:
         torch, table = self.torch, self._table
         if len(grads) != len(self.params):
             raise ValueError("AdamW: %d gradients for %d parameters" % (len(grads), len(self.params)))
-        gdt, keep = None, []
-        for i, (p, g) in enumerate(zip(self.params, grads)):
-            t = table[i]
-            if p.data_ptr() != t.param:
-                self._moved(i)
-            if g is None:
-                t.n = 0
-                continue
-            if gdt is None:
-                gdt = g.dtype
-            if g.dtype != gdt or g.device != self.device or g.numel() != self._live[i]:
-                raise ValueError("AdamW: gradient %d is %s of %d elements on %s; %s of %d on %s is needed"
-                                 % (i, g.dtype, g.numel(), g.device, gdt, self._live[i], self.device))
-            if not g.is_contiguous():
-                g = g.contiguous()
-                keep.append(g)
-            t.grad, t.n = g.data_ptr(), self._live[i]
+        at = [p.data_ptr() for p in self.params]
+        if at != self._at:
+            self._moved(at)
+        have = [g for g in grads if g is not None]
+        sizes = self._live if len(have) == len(grads) else [k for k, g in zip(self._live, grads) if g is not None]
+        dts = {g.dtype for g in have}
+        if len(dts) > 1 or [g.numel() for g in have] != sizes or {g.get_device() for g in have} - {self.device.index}:
+            for i, (g, k) in enumerate(zip(grads, self._live)):
+                if g is not None and (g.dtype != have[0].dtype or g.numel() != k or g.device != self.device):
+                    raise ValueError("AdamW: gradient %d is %s of %d elements on %s; %s of %d on %s is needed"
+                                     % (i, g.dtype, g.numel(), g.device, have[0].dtype, k, self.device))
+        if not all([g.is_contiguous() for g in have]):
+            grads = [g if g is None else g.contiguous() for g in grads]   # (kept until the launch)
+        if len(have) == len(grads):
+            self._columns[:, 1] = [g.data_ptr() for g in grads]
+            self._columns[:, 7] = self._live
+        else:
+            self._columns[:, 1] = [0 if g is None else g.data_ptr() for g in grads]
+            self._columns[:, 7] = [0 if g is None else k for g, k in zip(grads, self._live)]
         o = self._opts
-        o.grad_dtype = o.param_dtype if gdt is None else _lib.DTYPE_CODE.get(str(gdt)[6:], -1)
+        o.grad_dtype = _lib.DTYPE_CODE.get(str(dts.pop())[6:], -1) if dts else o.param_dtype
         if clip is not None and (clip.dtype != torch.float64 or clip.numel() != 2 or clip.device != self.device or not clip.is_contiguous()):
             raise ValueError("AdamW: clip is what grad_norm returns: a float64 tensor [norm, factor] on %s" % self.device)
         o.clip = None if clip is None else clip.data_ptr()
@@ -213,12 +220,13 @@ class AdamW:
         eng.check(rc)
         self.steps += 1
 
-    def _moved(self, i):
-        """parameter i was given other storage"""
-        p = self.params[i]
-        if p.device != self.device or str(p.dtype)[6:] != self.dtype or p.numel() != self._live[i] or not p.is_contiguous():
-            raise ValueError("AdamW: parameter %d was replaced by %s of %d elements on %s" % (i, p.dtype, p.numel(), p.device))
-        self._table[i].param = p.data_ptr()
+    def _moved(self, at):
+        """parameters were given other storage"""
+        for i, p in enumerate(self.params):
+            if p.device != self.device or str(p.dtype)[6:] != self.dtype or p.numel() != self._live[i] or not p.is_contiguous():
+                raise ValueError("AdamW: parameter %d was replaced by %s of %d elements on %s" % (i, p.dtype, p.numel(), p.device))
+        self._columns[:, 0] = at
+        self._at = at
 
     def moments(self, out=None):
         """[(m, v), ...]: the values of the moments, Float32 (Float64 for float64 parameters); out: pairs of tensors to write 8-bit
@@ -236,8 +244,7 @@ class AdamW:
                 if x.dtype != torch.float32 or x.numel() != self._live[i] or x.device != self.device or not x.is_contiguous():
                     raise ValueError("AdamW: output %d: float32 of %d elements on %s, contiguous, is needed" % (i, self._live[i], self.device))
         ms, vs = ((C.c_void_p * n)(*[pair[k].data_ptr() for pair in out]) for k in range(2))
-        for i, k in enumerate(self._live):
-            self._table[i].n = k
+        self._columns[:, 7] = self._live
         eng = _bound_engine(self.device)
         eng.check(eng.L.ude_adamw_moments_dev(eng.h, n, self._table, ms, vs))
         return out
