@@ -26,6 +26,13 @@ struct F32 {
     typedef float E;
     static __device__ float to(float x) { return x; }
     static __device__ E from(float x) { return x; }
+    // 16 k: four steps of four.  Which k a lane group feeds does not matter where both operands do the same.
+    static __device__ f4 mfma(s8 a, s8 b, f4 c) {
+        const f4 x = __builtin_bit_cast(f4, a), y = __builtin_bit_cast(f4, b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], c, 0, 0, 0);
+        return c;
+    }
 };
 struct F16 {
     typedef short E;  // 16-bit patterns: loads, LDS and the matrix instructions do not look at them
@@ -276,16 +283,9 @@ __global__ __launch_bounds__(256) void gemm_any(const Args a) {
                 for (int j = 0; j < 2; ++j) {
                     const E* pa = sA + (wm * 32 + i * 16 + r) * LD;
                     const E* pb = sB + (EPI == EPI_GATE ? j * 32 + wn * 16 + r : wn * 32 + j * 16 + r) * LD;
-                    if constexpr (sizeof(E) == 2) {
-                        acc[i][j] = T::mfma(*(const s8*)(pb + g * 8), *(const s8*)(pa + g * 8), acc[i][j]);
-                    } else {  // (a step of four k: the same k of both operands in every lane group, in any order)
+                    constexpr int V = 16 / (int)sizeof(E);
 #pragma unroll
-                        for (int kk = 0; kk < KS; kk += 16) {
-                            const f4 x = *(const f4*)(pb + kk + g * 4), w = *(const f4*)(pa + kk + g * 4);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], w[e], acc[i][j], 0, 0, 0);
-                        }
-                    }
+                    for (int kk = 0; kk < KS; kk += 4 * V) acc[i][j] = T::mfma(*(const s8*)(pb + kk + g * V), *(const s8*)(pa + kk + g * V), acc[i][j]);
                 }
         }
     }
@@ -302,16 +302,17 @@ __global__ __launch_bounds__(256) void gemm_any(const Args a) {
     }
 }
 
-// ---- the tile kernel of the 16-bit kinds ------------------------------------------------------------------------------------------
-// A BM x BN tile of C by NWM x NWN wavefronts; K in steps of 64 through LDS buffers that buffer_load .. lds fills 16 bytes a lane,
+// ---- the tile kernel -------------------------------------------------------------------------------------------------------------------
+// A BM x BN tile of C by NWM x NWN wavefronts; K in steps of 128 bytes (64 k of the 16-bit kinds, 32 of Float32) through LDS buffers that buffer_load .. lds fills 16 bytes a lane,
 // straight from memory: while step k is multiplied, the next ones are on their way.  What a descriptor's record count does not cover is
 // filled with zeros, so that edges cost no branches; a lane outside asks for OUTSIDE.
 //
 // LDS layouts (a 1 KB piece is one instruction of one wavefront, lane l at 16 l):
-//   "K" operand [row][64 k], 128 B a row: the 16-byte chunk c of row r lies at chunk c ^ (r & 7) -- 16 lanes that read chunk c of 16
-//       consecutive rows touch every bank once.
-//   "R" operand [64 k][W rows] (W = 128 or 64): read through ds_read_b64_tr_b16, which hands each lane four consecutive k of one row; the
-//       32-byte pair P of k-row k lies at P ^ spread(k), which spreads the 8 k-rows that are read together over the banks.
+//   "K" operand [row][128 B of k]: the 16-byte chunk c of row r lies at chunk c ^ (r & 7) -- 16 lanes that read chunk c of 16 consecutive
+//       rows touch every bank once.
+//   "R" operand [k][W rows] (W = 128 or 64): a k-row's groups of 16 rows lie at group ^ spread(k), which spreads what is read together over
+//       the banks.  16-bit kinds are read through ds_read_b64_tr_b16, which hands each lane four consecutive k of one row (8 k-rows read
+//       together), Float32 one by one (4 k-rows).
 constexpr unsigned OUTSIDE = 0x80000000u;
 typedef int i4 __attribute__((ext_vector_type(4)));
 
@@ -330,22 +331,23 @@ static __device__ inline void to_lds(unsigned at, unsigned off, i4 r, unsigned f
 }
 static __device__ inline unsigned lds_address(const void* p) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p; }
 
-template <int W>
+template <int ES, int W>
 static __device__ constexpr int spread(int k) {
-    return W == 128 ? (k & 3) | ((k >> 3) & 1) << 2 : ((k >> 1) & 1) | ((k >> 3) & 1) << 1;
+    return ES == 4 ? (k >> 2) & 3 : W == 128 ? (k & 3) | ((k >> 3) & 1) << 2 : ((k >> 1) & 1) | ((k >> 3) & 1) << 1;
 }
 
-// One operand of a tile: ROWS rows (of HALVES matrices, ROWS / HALVES each) by 64 k
+// One operand of a tile: ROWS rows (of HALVES matrices, ROWS / HALVES each) by 128 bytes of k
 template <class T, bool KC, int ROWS, int NW, int HALVES>
 struct Operand {
     typedef typename T::E E;
+    static constexpr int ES = sizeof(E), V = 16 / ES, KS = 128 / ES;   // elements of 16 bytes; k of a step
     static constexpr int N = ROWS / 8 / NW;                            // 1 KB pieces of a wavefront
     static constexpr int W = KC ? 0 : (ROWS / HALVES >= 128 ? 128 : 64);  // width of a sub-tile of an "R" operand
     static constexpr int BYTES = ROWS * 128;
     static_assert(N * 8 * NW == ROWS && N % HALVES == 0, "pieces");
     const char* base[HALVES];
     i4 rec[HALVES];
-    unsigned step[HALVES];  // bytes of 64 k
+    unsigned step[HALVES];  // bytes of a step
     unsigned off[N];
     int koff;  // "K": first k of this lane's chunks; "R": not used
 
@@ -353,8 +355,8 @@ struct Operand {
     __device__ inline void init(const void* const* p, const int64_t* ld, int row0, int rows, int k0, int K, int wave, int lane) {
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
-            base[h] = (const char*)p[h] + (KC ? (int64_t)row0 * ld[h] + k0 : (int64_t)k0 * ld[h] + row0) * 2;
-            rec[h] = records(base[h], (KC ? (int64_t)(rows - 1 - row0) * ld[h] + K - k0 : (int64_t)(K - 1 - k0) * ld[h] + rows - row0) * 2);
+            base[h] = (const char*)p[h] + (KC ? (int64_t)row0 * ld[h] + k0 : (int64_t)k0 * ld[h] + row0) * ES;
+            rec[h] = records(base[h], (KC ? (int64_t)(rows - 1 - row0) * ld[h] + K - k0 : (int64_t)(K - 1 - k0) * ld[h] + rows - row0) * ES);
             step[h] = KC ? 128 : 128 * (unsigned)ld[h];
         }
         koff = 0;
@@ -363,13 +365,13 @@ struct Operand {
             const int h = i / (N / HALVES), piece = (i % (N / HALVES)) * NW + wave;
             if constexpr (KC) {
                 const int r = piece * 8 + (lane >> 3);
-                koff = ((lane & 7) ^ (lane >> 3)) * 8;
-                off[i] = row0 + r < rows ? (unsigned)(r * (int)ld[h] * 2 + koff * 2) : OUTSIDE;
+                koff = ((lane & 7) ^ (lane >> 3)) * V;
+                off[i] = row0 + r < rows ? (unsigned)(r * (int)ld[h] * ES + koff * ES) : OUTSIDE;
             } else {
-                constexpr int PP = W / 8, RP = 512 / W;  // pieces of a sub-tile; k-rows of a piece
-                const int sub = piece / PP, k = (piece % PP) * RP + lane / (W / 8), u = lane % (W / 8);
-                const int r = sub * W + ((u >> 1) ^ spread<W>(k)) * 16 + (u & 1) * 8;
-                off[i] = row0 + r < rows ? (unsigned)(k * (int)ld[h] * 2 + r * 2) : OUTSIDE;
+                constexpr int PP = W / 8, UR = W / V, RP = 64 / UR, UG = 16 / V;  // pieces of a sub-tile; 16-byte units of a k-row; k-rows of a piece; units of 16 rows
+                const int sub = piece / PP, k = (piece % PP) * RP + lane / UR, u = lane % UR;
+                const int r = sub * W + ((u / UG) ^ spread<ES, W>(k)) * 16 + (u % UG) * V;
+                off[i] = row0 + r < rows ? (unsigned)(k * (int)ld[h] * ES + r * ES) : OUTSIDE;
             }
         }
     }
@@ -378,33 +380,39 @@ struct Operand {
         const int h = i / (N / HALVES);
         to_lds(at + (i * NW + wave) * 1024, off[i], rec[h], n * step[h]);
     }
-    // a last step of kleft < 64 k, `n` steps behind k0; where 8 does not divide kleft, a "K" operand goes element by element
+    // a last step of kleft < KS k, `n` steps behind k0; where it ends inside 16 bytes, a "K" operand goes element by element
     __device__ inline void tail(unsigned at, int wave, int lane, int n, int kleft, char* lds) {
-        if (!KC || kleft % 8 == 0) {
+        if (!KC || kleft % V == 0) {
 #pragma unroll
             for (int i = 0; i < N; ++i) to_lds(at + (i * NW + wave) * 1024, !KC || koff < kleft ? off[i] : OUTSIDE, rec[i / (N / HALVES)], n * step[i / (N / HALVES)]);
         } else {
+            typedef E EV __attribute__((ext_vector_type(V)));
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                s8 v = {};
+                EV v = {};
                 if (off[i] != OUTSIDE) {
                     const E* p = (const E*)(base[i / (N / HALVES)] + off[i] + n * step[i / (N / HALVES)]);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
+                    for (int e = 0; e < V; ++e)
                         if (koff + e < kleft) v[e] = p[e];
                 }
-                *(s8*)(lds + (i * NW + wave) * 1024 + lane * 16) = v;
+                *(EV*)(lds + (i * NW + wave) * 1024 + lane * 16) = v;
             }
         }
     }
-    // the 8 k of row `row` (a multiple of 16, plus lane & 15) that a lane feeds to the matrix instruction of k-half kk
+    // the 16 bytes of k of row `row` (a multiple of 16, plus lane & 15) that a lane feeds to the matrix instructions of k-half kk
     static __device__ inline s8 fragment(const char* lds, int row, int kk, int lane) {
         const int g = lane >> 4;
         if constexpr (KC) {
             return *(const s8*)(lds + (row + (lane & 15)) * 128 + (((kk * 4 + g) ^ (lane & 7)) << 4));
+        } else if constexpr (ES == 4) {
+            const int kr = kk * 16 + g * 4;
+            const float* p = (const float*)(lds + (row / W) * (W * 128)) + kr * W + (((row % W) >> 4) ^ spread<ES, W>(kr)) * 16 + (lane & 15);
+            const f4 x = {p[0], p[W], p[2 * W], p[3 * W]};
+            return __builtin_bit_cast(s8, x);
         } else {
             const int kr = g * 8 + ((lane & 15) >> 2);
-            const char* p = lds + (row / W) * (W * 128) + kr * (W * 2) + ((((row % W) >> 4) ^ spread<W>(kr)) << 5) + (lane & 3) * 8 + kk * 32 * (W * 2);
+            const char* p = lds + (row / W) * (W * 128) + kr * (W * 2) + ((((row % W) >> 4) ^ spread<ES, W>(kr)) << 5) + (lane & 3) * 8 + kk * 32 * (W * 2);
             typedef __attribute__((address_space(3))) s4* P;
             const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)p), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(p + 4 * (W * 2)));
             return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -443,6 +451,7 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
     constexpr int NT = BN / HALVES;  // output columns of a tile
     typedef Operand<T, AK, BM, NW, 1> OA;
     typedef Operand<T, BKc, BN, NW, HALVES> OB;
+    constexpr int KS = OA::KS;
     constexpr int BUFFERS = 2 * OB::BYTES + 3 * OA::BYTES;  // two of B, then three of A
     __shared__ __attribute__((aligned(1024))) char lds[BUFFERS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % NWM, wn = wave / NWM;
@@ -520,11 +529,11 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
         if (!BKc && (h ? HALVES == 2 || a.nseg == 2 : true) && (1 << 30) / (128 * a.p[z + h].ldb) < most) most = (1 << 30) / (128 * a.p[z + h].ldb);
     const int run = (int)most;
     // this part's steps out of the nseg * ksteps ones
-    const int ksteps = (a.K + 63) / 64, each = (a.nseg * ksteps + a.split - 1) / a.split;
+    const int ksteps = (a.K + KS - 1) / KS, each = (a.nseg * ksteps + a.split - 1) / a.split;
     for (int seg = 0; seg < a.nseg; ++seg) {
         const int lo = part * each - seg * ksteps, hi = lo + each;
-        const int64_t kend = hi >= ksteps ? a.K : (int64_t)hi * 64;
-        for (int64_t k0 = lo > 0 ? (int64_t)lo * 64 : 0; k0 < kend; k0 += (int64_t)run * 64) {
+        const int64_t kend = hi >= ksteps ? a.K : (int64_t)hi * KS;
+        for (int64_t k0 = lo > 0 ? (int64_t)lo * KS : 0; k0 < kend; k0 += (int64_t)run * KS) {
             {
                 const Product& s = a.p[a.nseg > 1 ? seg : z];
                 const void* pa[1] = {s.A};
@@ -534,7 +543,7 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
                 const int64_t lb[2] = {s.ldb, a.p[1].ldb};
                 ob.init(pb, lb, n0, q.N, (int)k0, a.K, wave, lane);
             }
-            const int left = (int)((kend - k0) / 64), full = left < run ? left : run, rest = left < run ? (int)((kend - k0) % 64) : 0;
+            const int left = (int)((kend - k0) / KS), full = left < run ? left : run, rest = left < run ? (int)((kend - k0) % KS) : 0;
             if (full) {
                 const int last = full - 1;
                 load_a(A0, 0), load_b(0, 0);

@@ -46,6 +46,7 @@ int vec(const void* p, int64_t ld, int e) { return (uintptr_t)p % 16 == 0 && ld 
 //   256 x 128, one per compute unit:    0.885                                   (two rounds of the same product: 311 us)
 //   128 x 128, two per compute unit:    1.04 for both, about 0.62 where one has the unit alone   (365 us)
 //   32 x 128, three per compute unit:   for few rows
+// Float32 is bound by its matrix instructions (1/16 of the 16-bit rate) whatever the tile: 128 x 128, 7.4 a step of 32 k.
 // The larger the tile, the less is read again; the smaller, the less of the last round stands idle.  EPI_PULL reads two floats and writes
 // three values per element between the products: 53, 33 and 20 us a round, hidden by the other workgroup's products where two share a unit.
 // Where tiles are few and K is long, K is cut into parts whose sums go through memory (3 TB/s) and one more launch.
@@ -55,7 +56,7 @@ struct Plan {
     int64_t big, all;  // tiles of the first launch; of all
     int split;         // 2, 4: parts of K
 };
-Plan plan(const Args& a, int epi, bool ak) {
+Plan plan(const Args& a, int epi, bool ak, int es) {
     const int H = epi == EPI_GATE ? 2 : 1;
     bool few = ak;  // (32 x 128 reads A by rows)
     for (int i = 0; i < a.nprod; ++i) few = few && a.p[i].M <= 32;
@@ -64,10 +65,10 @@ Plan plan(const Args& a, int epi, bool ak) {
         for (int i = 0; i < a.nprod; ++i) n += (int64_t)((a.p[i].M + bm - 1) / bm) * ((a.p[i].N + bn / H - 1) / (bn / H));
         return n;
     };
-    const int total = a.nseg * ((a.K + 63) / 64);
+    const int total = a.nseg * ((a.K + 128 / es - 1) / (128 / es));
     const bool pull = epi == EPI_PULL;
-    const double steps = total + 3, e2 = pull ? 20 : 8;
-    const double r0 = steps * 1.55 + (pull ? 53 : 10), r1 = steps * 0.885 + (pull ? 33 : 8), r2 = steps * 1.04 + e2;
+    const double steps = total + 3, e2 = pull ? 20 : 8, c2 = es == 4 ? 7.4 : 1.04;
+    const double r0 = steps * 1.55 + (pull ? 53 : 10), r1 = steps * 0.885 + (pull ? 33 : 8), r2 = steps * c2 + e2;
     auto small = [&](int64_t n, double r) {
         const int64_t whole = n / (2 * CUS), rest = n % (2 * CUS);
         return whole * r + (rest == 0 ? 0 : rest <= CUS ? 0.62 * r : r);
@@ -81,10 +82,11 @@ Plan plan(const Args& a, int epi, bool ak) {
     }
     double least = small(n2, r2);
     for (int s = 2; s * n2 <= MOST_PARTS && s * 2 <= total; ++s) {
-        const double cost = small(n2 * s, ((total + s - 1) / s + 3) * 1.04) + n2 * s * (2 * 65536 / 3e6) + e2 + 4;
+        const double cost = small(n2 * s, ((total + s - 1) / s + 3) * c2) + n2 * s * (2 * 65536 / 3e6) + e2 + 4;
         if (cost < least) least = cost, best.split = s;
     }
     const double cost[3] = {(n0 + CUS - 1) / CUS * r0, (n1 + CUS - 1) / CUS * r1, n0 > CUS && rest ? n0 / CUS * r0 + small(4 * rest, r2) + 4 : 1e30};
+    if (es == 4) return best;
     if (cost[0] < least) least = cost[0], best = {0, n0, n0, 1};
     if (cost[1] < least) least = cost[1], best = {1, n1, n1, 1};
     if (cost[2] < least) least = cost[2], best = {3, n0 - rest, n0, 1};
@@ -97,22 +99,23 @@ int64_t part_bytes(int64_t M, int64_t N, int64_t steps, int n) {
 }
 static_assert(MOST_PARTS * 65536 / 2 >= MOST_PARTS_32 * 16384, "parts of 32 rows need less");
 
-// a row of 16-bit elements starts on a 4-byte boundary, and a tile's offsets fit 31 bits
-bool tileable(const void* p, int64_t ld) { return (uintptr_t)p % 4 == 0 && ld % 2 == 0 && ld < (1 << 22); }
+// a row starts on a 4-byte boundary, and a tile's offsets fit 31 bits
+bool tileable(const void* p, int64_t ld, int e) { return (uintptr_t)p % 4 == 0 && ld * e % 4 == 0 && ld * e < (1 << 23); }
 
 template <class T, int EPI, bool AK, bool BKc>
 int launch3(ude_ctx* c, Args a, bool tile) {
     a.split = 1;
-    if constexpr (sizeof(typename T::E) == 2) {
-        const Plan p = plan(a, EPI, AK);
+    constexpr bool WIDE = sizeof(typename T::E) == 2;  // (the tiles of 256 rows)
+    {
+        const Plan p = plan(a, EPI, AK, sizeof(typename T::E));
         if (tile && p.big < 1 << 22 && p.all < 1 << 22) {
             a.split = p.split;
             const dim3 grid((unsigned)(p.big * p.split)), block(256);
-            if (p.which == 0 || p.which == 3)
-                hipLaunchKernelGGL((gemm_tile<T, EPI, AK, BKc, 256, 256, 2, 2, 1>), grid, block, 0, c->stream, a);
-            else if (p.which == 1)
-                hipLaunchKernelGGL((gemm_tile<T, EPI, AK, BKc, 256, 128, 2, 2, 1>), grid, block, 0, c->stream, a);
-            else if (p.which == 2)
+            if (WIDE && (p.which == 0 || p.which == 3)) {
+                if constexpr (WIDE) hipLaunchKernelGGL((gemm_tile<T, EPI, AK, BKc, 256, 256, 2, 2, 1>), grid, block, 0, c->stream, a);
+            } else if (WIDE && p.which == 1) {
+                if constexpr (WIDE) hipLaunchKernelGGL((gemm_tile<T, EPI, AK, BKc, 256, 128, 2, 2, 1>), grid, block, 0, c->stream, a);
+            } else if (p.which == 2)
                 hipLaunchKernelGGL((gemm_tile<T, EPI, AK, BKc, 128, 128, 2, 2, 2>), grid, block, 0, c->stream, a);
             else if constexpr (AK)
                 hipLaunchKernelGGL((gemm_tile<T, EPI, AK, BKc, 32, 128, 1, 4, 3>), grid, block, 0, c->stream, a);
@@ -161,9 +164,9 @@ int launch(ude_ctx* c, int dtype, Args a, bool ak, bool bk) {
         p.vecC = (uintptr_t)p.C % (4 * e) == 0 && p.ldc % 4 == 0;
         // gate and up are rows of N floats; dg, du, h lie in the workspace, rows of a multiple of 8
         if (EPI != EPI_STORE && a.gate && (p.N % 4 || (uintptr_t)a.gate % 16 || (uintptr_t)a.up % 16)) p.vecC = 0;
-        tile = tile && tileable(p.A, p.lda) && tileable(p.B, p.ldb);
+        tile = tile && tileable(p.A, p.lda, e) && tileable(p.B, p.ldb, e);
     }
-    if (dtype == UDE_DT_F32) return launch2<F32, EPI>(c, a, ak, bk, false);
+    if (dtype == UDE_DT_F32) return launch2<F32, EPI>(c, a, ak, bk, tile);
     if (dtype == UDE_DT_F16) return launch2<F16, EPI>(c, a, ak, bk, tile);
     return launch2<BF16, EPI>(c, a, ak, bk, tile);
 }
@@ -182,8 +185,8 @@ Space space(const ude_gated_ffn_desc* d, bool pullback) {
     s.h = pullback ? up256(d->T * s.ldg * e) : 0;
     s.part = s.h + up256(d->T * s.ldh * e);
     s.all = s.part;
-    if (e == 2 && d->T) {  // (Float32 leaves no parts)
-        auto steps = [](int64_t k) { return (k + 63) / 64; };
+    if (d->T) {
+        auto steps = [e](int64_t k) { return (k + 128 / e - 1) / (128 / e); };
         const int64_t wide = d->D > d->O ? d->D : d->O;
         const int64_t a = pullback ? part_bytes(d->T, d->F, steps(d->O), 1) : part_bytes(d->T, d->F, steps(d->D), 1);
         const int64_t b = pullback ? part_bytes(d->T, d->D, 2 * steps(d->F), 1) : part_bytes(d->T, d->O, steps(d->F), 1);
