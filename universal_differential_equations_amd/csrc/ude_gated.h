@@ -132,6 +132,7 @@ struct Args {
     // sums of tile t and part s go to part[(t * split + s) * tile size] and join_parts adds them up
     int first, quarters, split;
     float* part;
+    int64_t room;  // bytes there
     float *gate, *up;     // EPI_GATE: stored if not NULL; EPI_PULL: read; leading dimension N
     void *dg, *du, *h;    // EPI_PULL: dg and du with leading dimension p[0].ldc, h with ldh
     int64_t ldh;
@@ -593,7 +594,7 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
     // epilogue: 32 rows of a wavefront at a time through LDS, so that the code of finish() stands in a loop and a row's lanes store side by
     // side, up to four stores a turn.  (The rows are four floats longer than they need to be: 8 lanes that write 16 bytes of 8 rows touch every
     // bank once.)
-    constexpr int COLS = BN / NWN, LDC = COLS + 4, CT = COLS / HALVES, TURN = 32 * CT / 4 < 256 ? 32 * CT / 4 / 64 : 4;
+    constexpr int COLS = BN / NWN, LDC = COLS + 4, CT = COLS / HALVES, MOST = EPI == EPI_PULL && BM == 256 ? 8 : 4, TURN = 32 * CT / 4 < 64 * MOST ? 32 * CT / 4 / 64 : MOST;
     static_assert(NW * 32 * LDC * 4 <= BUFFERS && 32 * CT / 4 % (64 * TURN) == 0, "epilogue");
     float* mine = (float*)lds + wave * 32 * LDC;
 #pragma unroll 1

@@ -41,100 +41,133 @@ int misaligned(const void* p, int e) { return (uintptr_t)p % e != 0; }
 
 int vec(const void* p, int64_t ld, int e) { return (uintptr_t)p % 16 == 0 && ld * e % 16 == 0; }
 
-// Tiles of the 16-bit kinds on the 256 compute units of an MI355X.  Costs in microseconds, measured at long K:
-//   256 x 256, one per compute unit:    1.55 a step of 64 k, then the epilogue  (4096 x 4096 x 11264: 271 us = 1395 TFLOP/s)
-//   256 x 128, one per compute unit:    0.885                                   (two rounds of the same product: 311 us)
-//   128 x 128, two per compute unit:    1.04 for both, about 0.62 where one has the unit alone   (365 us)
-//   32 x 128, three per compute unit:   for few rows
-// Float32 is bound by its matrix instructions (1/16 of the 16-bit rate) whatever the tile: 128 x 128, 7.4 a step of 32 k.
-// The larger the tile, the less is read again; the smaller, the less of the last round stands idle.  EPI_PULL reads two floats and writes
-// three values per element between the products: 53, 33 and 20 us a round, hidden by the other workgroup's products where two share a unit.
-// Where tiles are few and K is long, K is cut into parts whose sums go through memory (3 TB/s) and one more launch.
-constexpr int CUS = 256, MOST_PARTS = 2 * CUS, MOST_PARTS_32 = 3 * CUS;
-struct Plan {
-    int which;         // 0: 256 x 256, 1: 256 x 128, 2: 128 x 128, 3: whole rounds of 256 x 256, the rest as quarters, 4: 32 x 128
-    int64_t big, all;  // tiles of the first launch; of all
-    int split;         // 2, 4: parts of K
+// Tiles on the 256 compute units of an MI355X: microseconds that a step of 128 bytes of k takes with 1, 2, 3 workgroups on a compute unit, and
+// the start and epilogue of a round, as measured (kernel times over products of 64 x 512 x 1408 to 4096 x 4096 x 11264).
+//   256 x 256: the least that is read again: 4096 x 4096 x 11264 in 271 us = 1395 TFLOP/s; 256 x 128: 311 us; 128 x 128: 365 us.
+//   The smaller ones leave less of the last round idle; a step costs them 0.4 to 0.5 however little there is in it (barrier, LDS, the loads'
+//   way), so that 64 and 32 rows are for small products, and for Float32, whose matrix instructions (1/16 of the 16-bit rate) bound it with
+//   any tile.
+// EPI_GATE writes ten bytes an element at the end, EPI_PULL reads eight and writes six.  Where tiles are few and K is long, K is cut into
+// parts whose sums go through memory (3 TB/s) and one more launch.
+constexpr int CUS = 256;
+constexpr int64_t MOST_PART_BYTES = (int64_t)2 * CUS * 128 * 128 * 4;
+enum { T256 = 0, T256x128 = 1, T128 = 2, T64 = 3, T32 = 4, TILES = 5 };
+struct Tile {
+    int bm, bn, bn_gate;             // EPI_GATE: of which half are output columns
+    int slots, slots_gate;           // workgroups of a compute unit
+    double step[3], gate[3];         // 16-bit kinds; EPI_GATE's where its tile is another
+    double step32[3], gate32[3];     // Float32 (0: there is none)
+    double end[3];                   // EPI_STORE, EPI_GATE, EPI_PULL
 };
-Plan plan(const Args& a, int epi, bool ak, int es) {
-    const int H = epi == EPI_GATE ? 2 : 1;
-    bool few = ak;  // (32 x 128 reads A by rows)
-    for (int i = 0; i < a.nprod; ++i) few = few && a.p[i].M <= 32;
-    auto tiles = [&](int bm, int bn) {
-        int64_t n = 0;
-        for (int i = 0; i < a.nprod; ++i) n += (int64_t)((a.p[i].M + bm - 1) / bm) * ((a.p[i].N + bn / H - 1) / (bn / H));
-        return n;
-    };
+constexpr Tile TILE[TILES] = {
+    {256, 256, 256, 1, 1, {1.48}, {1.48}, {}, {}, {6, 17, 42}},
+    {256, 128, 128, 1, 1, {0.87}, {0.87}, {}, {}, {5, 10, 25}},
+    {128, 128, 128, 2, 2, {0.48, 1.02}, {0.48, 1.02}, {1.95, 3.8}, {1.95, 3.8}, {6, 9, 17}},
+    {64, 64, 128, 3, 2, {0.41, 0.43, 0.62}, {0.45, 0.66}, {0.54, 1.08, 1.6}, {1.08, 2.1}, {4, 6, 7}},
+    {32, 128, 128, 3, 3, {0.46, 0.50, 0.65}, {0.46, 0.50, 0.65}, {0.55, 1.1, 1.65}, {0.55, 1.1, 1.65}, {4, 5, 7}}};
+struct Plan {
+    int which, split;  // tile; parts of K
+    int quarters;      // T256: whole rounds of them, the rest as quarters, cut into so many parts of K (0: no such rest)
+    int64_t big, all;  // tiles of the first launch; of all
+};
+int64_t tiles_of(const Args& a, int epi, int which) {
+    const int bm = TILE[which].bm, bn = epi == EPI_GATE ? TILE[which].bn_gate / 2 : TILE[which].bn;
+    int64_t n = 0;
+    for (int i = 0; i < a.nprod; ++i) n += (int64_t)((a.p[i].M + bm - 1) / bm) * ((a.p[i].N + bn - 1) / bn);
+    return n;
+}
+int slots_of(int which, int epi) { return epi == EPI_GATE ? TILE[which].slots_gate : TILE[which].slots; }
+double tiles_cost(int which, int epi, int es, int64_t n, double steps) {
+    const Tile& t = TILE[which];
+    const double* c = epi == EPI_GATE ? (es == 4 ? t.gate32 : t.gate) : (es == 4 ? t.step32 : t.step);
+    const int slots = slots_of(which, epi);
+    const int64_t whole = n / (slots * CUS), rest = (n % (slots * CUS) + CUS - 1) / CUS;
+    return whole * (steps * c[slots - 1] + t.end[epi]) + (rest ? steps * c[rest - 1] + t.end[epi] : 0);
+}
+int64_t part_size(int which, int epi) { return (int64_t)TILE[which].bm * (epi == EPI_GATE ? TILE[which].bn_gate : TILE[which].bn) * 4; }
+// the least that n tiles cost with K whole or cut into parts; room: bytes of workspace for them
+double cut(int which, int epi, int es, int64_t n, int total, int64_t room, int* parts) {
+    double least = tiles_cost(which, epi, es, n, total);
+    *parts = 1;
+    for (int s = 2; s * n <= slots_of(which, epi) * CUS && s * n * part_size(which, epi) <= room && s * 2 <= total; ++s) {
+        const double c = tiles_cost(which, epi, es, n * s, (total + s - 1) / s) + n * s * part_size(which, epi) * (2 / 3e6) + 6;
+        if (c < least) least = c, *parts = s;
+    }
+    return least;
+}
+Plan plan(const Args& a, int epi, bool ak, int es, int64_t room) {
     const int total = a.nseg * ((a.K + 128 / es - 1) / (128 / es));
-    const bool pull = epi == EPI_PULL;
-    const double steps = total + 3, e2 = pull ? 20 : 8, c2 = es == 4 ? 7.4 : 1.04;
-    const double r0 = steps * 1.55 + (pull ? 53 : 10), r1 = steps * 0.885 + (pull ? 33 : 8), r2 = steps * c2 + e2;
-    auto small = [&](int64_t n, double r) {
-        const int64_t whole = n / (2 * CUS), rest = n % (2 * CUS);
-        return whole * r + (rest == 0 ? 0 : rest <= CUS ? 0.62 * r : r);
-    };
-    const int64_t n0 = tiles(256, 256), n1 = tiles(256, 128), n2 = tiles(few ? 32 : 128, 128), rest = n0 % CUS;
-    Plan best = {few ? 4 : 2, n2, n2, 1};
+    bool few = ak;
+    for (int i = 0; i < a.nprod; ++i) few = few && a.p[i].M <= 32;
     if (few) {  // bound by reading B: parts until every compute unit has three workgroups, each of 4 steps at least
-        const int64_t most = MOST_PARTS_32 / n2 < total / 4 ? MOST_PARTS_32 / n2 : total / 4;
-        if (most > 1) best.split = (int)most;
-        return best;
+        const int64_t n = tiles_of(a, epi, T32), fit = room / (n * part_size(T32, epi));
+        int64_t most = 3 * CUS / n < total / 4 ? 3 * CUS / n : total / 4;
+        most = most < fit ? most : fit;
+        return {T32, most > 1 ? (int)most : 1, 0, n, n};
     }
-    double least = small(n2, r2);
-    for (int s = 2; s * n2 <= MOST_PARTS && s * 2 <= total; ++s) {
-        const double cost = small(n2 * s, ((total + s - 1) / s + 3) * c2) + n2 * s * (2 * 65536 / 3e6) + e2 + 4;
-        if (cost < least) least = cost, best.split = s;
+    Plan best{};
+    double least = 1e30;
+    for (int which = 0; which < TILES; ++which) {
+        if ((es == 4 && TILE[which].step32[0] == 0) || (which == T32 && !ak)) continue;
+        const int64_t n = tiles_of(a, epi, which);
+        const double cost = tiles_cost(which, epi, es, n, total);
+        if (cost < least) least = cost, best = {which, 1, 0, n, n};
+        if (which == T256 && n > CUS && n % CUS) {
+            const int64_t rest = n % CUS;
+            int parts;
+            const double c = tiles_cost(T256, epi, es, n - rest, total) + cut(T128, epi, es, 4 * rest, total, room, &parts) + 2;
+            if (c < least) least = c, best = {T256, 1, parts, n - rest, n};
+        }
+        if (which < T128) continue;
+        int parts;
+        const double c = cut(which, epi, es, n, total, room, &parts);
+        if (c < least) least = c, best = {which, parts, 0, n, n};
     }
-    const double cost[3] = {(n0 + CUS - 1) / CUS * r0, (n1 + CUS - 1) / CUS * r1, n0 > CUS && rest ? n0 / CUS * r0 + small(4 * rest, r2) + 4 : 1e30};
-    if (es == 4) return best;
-    if (cost[0] < least) least = cost[0], best = {0, n0, n0, 1};
-    if (cost[1] < least) least = cost[1], best = {1, n1, n1, 1};
-    if (cost[2] < least) least = cost[2], best = {3, n0 - rest, n0, 1};
     return best;
 }
 // no product of these sizes, nor some of `n` such products side by side, leaves more bytes of parts than this
 int64_t part_bytes(int64_t M, int64_t N, int64_t steps, int n) {
-    const int64_t all = n * ((M + 127) / 128) * ((N + 63) / 64) * (steps / 2);
-    return (all < MOST_PARTS ? all : MOST_PARTS) * 65536;
+    const int64_t all = n * ((M + 127) / 128) * ((N + 63) / 64) * (steps / 2);  // (part bytes of a tile go with its area: the largest tile's)
+    return all < MOST_PART_BYTES / 65536 ? all * 65536 : MOST_PART_BYTES;
 }
-static_assert(MOST_PARTS * 65536 / 2 >= MOST_PARTS_32 * 16384, "parts of 32 rows need less");
 
 // a row starts on a 4-byte boundary, and a tile's offsets fit 31 bits
 bool tileable(const void* p, int64_t ld, int e) { return (uintptr_t)p % 4 == 0 && ld * e % 4 == 0 && ld * e < (1 << 23); }
 
 template <class T, int EPI, bool AK, bool BKc>
 int launch3(ude_ctx* c, Args a, bool tile) {
-    a.split = 1;
-    constexpr bool WIDE = sizeof(typename T::E) == 2;  // (the tiles of 256 rows)
-    {
-        const Plan p = plan(a, EPI, AK, sizeof(typename T::E));
-        if (tile && p.big < 1 << 22 && p.all < 1 << 22) {
-            a.split = p.split;
-            const dim3 grid((unsigned)(p.big * p.split)), block(256);
-            if (WIDE && (p.which == 0 || p.which == 3)) {
-                if constexpr (WIDE) hipLaunchKernelGGL((gemm_tile<T, EPI, AK, BKc, 256, 256, 2, 2, 1>), grid, block, 0, c->stream, a);
-            } else if (WIDE && p.which == 1) {
-                if constexpr (WIDE) hipLaunchKernelGGL((gemm_tile<T, EPI, AK, BKc, 256, 128, 2, 2, 1>), grid, block, 0, c->stream, a);
-            } else if (p.which == 2)
-                hipLaunchKernelGGL((gemm_tile<T, EPI, AK, BKc, 128, 128, 2, 2, 2>), grid, block, 0, c->stream, a);
-            else if constexpr (AK)
-                hipLaunchKernelGGL((gemm_tile<T, EPI, AK, BKc, 32, 128, 1, 4, 3>), grid, block, 0, c->stream, a);
-            HIPCHK(c, hipGetLastError());
-            if (p.which == 3) {
-                a.first = (int)p.big, a.quarters = 1;
-                hipLaunchKernelGGL((gemm_tile<T, EPI, AK, BKc, 128, 128, 2, 2, 2>), dim3((unsigned)(4 * (p.all - p.big))), block, 0, c->stream, a);
-                HIPCHK(c, hipGetLastError());
-            }
-            if (p.split > 1) {
-                if (p.which == 2)
-                    hipLaunchKernelGGL((join_parts<T, EPI, 128, 128, 2, 2>), dim3((unsigned)p.big, 4), block, 0, c->stream, a);
-                else
-                    hipLaunchKernelGGL((join_parts<T, EPI, 32, 128, 1, 4>), dim3((unsigned)p.big, 2), block, 0, c->stream, a);
-                HIPCHK(c, hipGetLastError());
-            }
-            return UDE_OK;
+    const Plan p = plan(a, EPI, AK, sizeof(typename T::E), a.room);
+    if (tile && p.big * p.split < 1 << 22 && p.all < 1 << 22) {
+        constexpr bool GATE = EPI == EPI_GATE;
+        a.split = p.split;
+        const dim3 grid((unsigned)(p.big * p.split)), block(256);
+        auto go = [&](auto kernel, dim3 g) { hipLaunchKernelGGL(kernel, g, block, 0, c->stream, a); };
+        if constexpr (sizeof(typename T::E) == 2) {
+            if (p.which == T256) go(gemm_tile<T, EPI, AK, BKc, 256, 256, 2, 2, 1>, grid);
+            if (p.which == T256x128) go(gemm_tile<T, EPI, AK, BKc, 256, 128, 2, 2, 1>, grid);
         }
+        if (p.which == T128) go(gemm_tile<T, EPI, AK, BKc, 128, 128, 2, 2, 2>, grid);
+        if (p.which == T64) go(gemm_tile<T, EPI, AK, BKc, 64, GATE ? 128 : 64, 2, 2, GATE ? 2 : 3>, grid);
+        if constexpr (AK)
+            if (p.which == T32) go(gemm_tile<T, EPI, AK, BKc, 32, 128, 1, 4, 3>, grid);
+        HIPCHK(c, hipGetLastError());
+        if (p.quarters) {
+            const unsigned rest = (unsigned)(4 * (p.all - p.big));
+            a.first = (int)p.big, a.quarters = 1, a.split = p.quarters;
+            go(gemm_tile<T, EPI, AK, BKc, 128, 128, 2, 2, 2>, dim3(rest * p.quarters));
+            HIPCHK(c, hipGetLastError());
+            if (p.quarters > 1) go(join_parts<T, EPI, 128, 128, 2, 2>, dim3(rest, 4));
+            HIPCHK(c, hipGetLastError());
+        }
+        if (p.split > 1) {
+            if (p.which == T128) go(join_parts<T, EPI, 128, 128, 2, 2>, dim3((unsigned)p.big, 4));
+            if (p.which == T64) go(join_parts<T, EPI, 64, GATE ? 128 : 64, 2, 2>, dim3((unsigned)p.big, 2));
+            if (p.which == T32) go(join_parts<T, EPI, 32, 128, 1, 4>, dim3((unsigned)p.big, 2));
+            HIPCHK(c, hipGetLastError());
+        }
+        return UDE_OK;
     }
+    a.split = 1;
     constexpr int NT = EPI == EPI_GATE ? 32 : 64;
     int64_t n = 0;
     for (int i = 0; i < a.nprod; ++i) {
@@ -222,12 +255,12 @@ extern "C" int ude_gated_ffn_forward_dev(ude_ctx* c, const ude_gated_ffn_desc* d
     const bool rows = d->w_order == 1;
     const int T = (int)d->T, D = (int)d->D, F = (int)d->F, O = (int)d->O;
     Args a{};
-    a.nprod = a.nseg = 1, a.K = D, a.act = d->act, a.gate = gate, a.up = up, a.part = (float*)((char*)ws + sp.part);
+    a.nprod = a.nseg = 1, a.K = D, a.act = d->act, a.gate = gate, a.up = up, a.part = (float*)((char*)ws + sp.part), a.room = sp.all - sp.part;
     a.p[0] = {x, wg, ws, d->ldx, d->ldg, wld(F), T, F};
     a.p[1] = {x, wu, ws, d->ldx, d->ldu, wld(F), T, F};
     if (int rc = launch<EPI_GATE>(c, d->dtype, a, true, rows)) return rc;
     Args b{};
-    b.nprod = b.nseg = 1, b.K = F, b.part = a.part;
+    b.nprod = b.nseg = 1, b.K = F, b.part = a.part, b.room = a.room;
     b.p[0] = {ws, wd, y, wld(F), d->ldd, d->ldy, T, O};
     return launch<EPI_STORE>(c, d->dtype, b, true, rows);
 }
@@ -253,16 +286,17 @@ extern "C" int ude_gated_ffn_backward_dev(ude_ctx* c, const ude_gated_ffn_desc* 
     char* du = dg + ldh * e;
     char* h = (char*)ws + sp.h;
     float* part = (float*)((char*)ws + sp.part);
+    const int64_t room = sp.all - sp.part;
     if (T) {
         Args a{};
         a.nprod = a.nseg = 1, a.K = O, a.act = d->act;
         a.p[0] = {dy, wd, dg, d->ldy, d->ldd, ldg, T, F};
-        a.gate = (float*)gate, a.up = (float*)up, a.dg = dg, a.du = du, a.h = h, a.ldh = ldh, a.part = part;
+        a.gate = (float*)gate, a.up = (float*)up, a.dg = dg, a.du = du, a.h = h, a.ldh = ldh, a.part = part, a.room = room;
         if (int rc = launch<EPI_PULL>(c, d->dtype, a, true, !rows)) return rc;
     }
     if (dx && T) {
         Args a{};
-        a.nprod = 1, a.nseg = 2, a.K = F, a.part = part;
+        a.nprod = 1, a.nseg = 2, a.K = F, a.part = part, a.room = room;
         a.p[0] = {dg, wg, dx, ldg, d->ldg, D, T, D};
         a.p[1] = {du, wu, dx, ldg, d->ldu, D, T, D};
         if (int rc = launch<EPI_STORE>(c, d->dtype, a, true, !rows)) return rc;
@@ -270,7 +304,7 @@ extern "C" int ude_gated_ffn_backward_dev(ude_ctx* c, const ude_gated_ffn_desc* 
     // gradients of the weights in the order of the weights, side by side in one launch: the axis whose elements are adjacent is n.
     // (T = 0: an empty sum, zeros.)
     Args a{};
-    a.nseg = 1, a.K = T, a.part = part;
+    a.nseg = 1, a.K = T, a.part = part, a.room = room;
     auto add = [&](const void* out, const void* in, int64_t ldout, int64_t ldin, void* grad, int no, int ni) {
         if (!grad) return;
         if (rows)
