@@ -169,9 +169,9 @@ def test_output_rows_with_gaps_are_left_alone():
         b = _Block(x, wg, wu, wd, "swish")
         b.D.ldy = O + 6
         y = torch.full((T + 1, O + 6), 7.0, dtype=torch.bfloat16, device="cuda")
-        ws = b.workspace(0)
+        ws, size = b.workspace(0)
         b.bind()
-        b.eng.check(b.eng.L.ude_gated_ffn_forward_dev(b.eng.h, C.byref(b.D), *(t.data_ptr() for t in (x, wg, wu, wd, y)), None, None, ws.data_ptr(), ws.numel()))
+        b.eng.check(b.eng.L.ude_gated_ffn_forward_dev(b.eng.h, C.byref(b.D), *(t.data_ptr() for t in (x, wg, wu, wd, y)), None, None, ws.data_ptr(), size))
         assert bool((y[:, O:] == 7).all()) and bool((y[T] == 7).all())
         assert R.within(y[:T, :O], R.gated(x, wg, wu, wd, "swish")["y"]) <= 1
         assert _lib.GATE["swish"] == b.D.act

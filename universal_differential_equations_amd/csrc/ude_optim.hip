@@ -41,7 +41,7 @@ constexpr int64_t ADAM_CHUNK = 4096;    // elements of one workgroup that writes
 constexpr int64_t ADAM8_CHUNK = 4096;   // with 8-bit moments: 16 a thread
 constexpr int64_t ADAM32_CHUNK = 1024;  // with 32-bit moments: 4 a thread
 constexpr int64_t NORM_CHUNK = 4096;
-constexpr int NORM_BLOCKS = 2048;
+constexpr int NORM_BLOCKS = 2048, NORM_ONE = 64;
 constexpr int64_t MOST_CHUNKS = (int64_t)1 << 23;                   // of one launch: 256 threads each, fewer than 2^32
 constexpr int64_t MOST_ELEMENTS = MOST_CHUNKS * ADAM32_CHUNK;       // of one tensor
 
@@ -398,43 +398,54 @@ struct NormArgs {
 };
 static_assert(sizeof(NormArgs) <= 4096, "kernel arguments");
 
-// sum over the workgroup in a fixed order; valid in thread 0
+// sum over the workgroup (up to 16 wavefronts) in a fixed order; valid in thread 0
 __device__ inline double block_sum(double x) {
-    __shared__ double s[4];
+    __shared__ double s[16];
 #pragma unroll
     for (int d = 32; d; d /= 2) x += __shfl_down(x, d, 64);
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = x;
     __syncthreads();
-    return s[0] + s[1] + s[2] + s[3];
+    double all = 0;
+    for (unsigned i = 0; i < blockDim.x / 64; ++i) all += s[i];
+    return all;
+}
+
+// thread t of 256 adds its 16 elements of chunk c: 16-byte loads side by side where the tensor allows it, all of them before the first use
+template <class G>
+__device__ inline void add_chunk(const NormArgs& a, int c, int t, double* sum) {
+    typedef typename G::E E;
+    constexpr int V = 16 / sizeof(E);
+    const int k = tensor_of(a, c);
+    const int64_t at = (int64_t)(c - a.first[k]) * NORM_CHUNK;
+    const int64_t end = a.n[k] < at + NORM_CHUNK ? a.n[k] : at + NORM_CHUNK;
+    const E* g = (const E*)a.g[k];
+    E x[16];
+    if (end == at + NORM_CHUNK && fits<V>(g)) {
+#pragma unroll
+        for (int j = 0; j < 16 / V; ++j) get<V>(g + at + j * 256 * V + t * V, x + j * V);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int64_t i = at + j * 256 + t;
+            x[j] = i < end ? g[i] : (E)0;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const double y = (double)(typename G::W)x[j];
+        sum[j % 4] = fma(y, y, sum[j % 4]);
+    }
+}
+__device__ inline void write_norm(double sum, double max_norm, double* out) {
+    const double norm = sqrt(sum);
+    out[0] = norm;
+    out[1] = !(max_norm > 0) ? (norm != norm ? norm : 1) : norm <= max_norm ? 1 : max_norm / norm;
 }
 
 template <class G>
 __global__ __launch_bounds__(256) void norm_part_kernel(const NormArgs a) {
-    typedef typename G::E E;
-    constexpr int V = 16 / sizeof(E);
     double sum[4] = {};
-    for (int c = (int)blockIdx.x; c < a.chunks; c += (int)gridDim.x) {
-        const int k = tensor_of(a, c);
-        const int64_t at = (int64_t)(c - a.first[k]) * NORM_CHUNK;
-        const int64_t end = a.n[k] < at + NORM_CHUNK ? a.n[k] : at + NORM_CHUNK;
-        const E* g = (const E*)a.g[k];
-        E x[16];
-        if (end == at + NORM_CHUNK && fits<V>(g)) {
-#pragma unroll
-            for (int j = 0; j < 16 / V; ++j) get<V>(g + at + j * 256 * V + threadIdx.x * V, x + j * V);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const int64_t i = at + j * 256 + threadIdx.x;
-                x[j] = i < end ? g[i] : (E)0;
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const double y = (double)(typename G::W)x[j];
-            sum[j % 4] = fma(y, y, sum[j % 4]);
-        }
-    }
+    for (int c = (int)blockIdx.x; c < a.chunks; c += (int)gridDim.x) add_chunk<G>(a, c, threadIdx.x, sum);
     const double all = block_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
     if (threadIdx.x == 0) a.part[blockIdx.x] = all;
 }
@@ -443,11 +454,16 @@ __global__ __launch_bounds__(256) void norm_join_kernel(const double* part, int 
     double sum = 0;
     for (int i = threadIdx.x; i < n; i += 256) sum += part[i];
     sum = block_sum(sum);
-    if (threadIdx.x == 0) {
-        const double norm = sqrt(sum);
-        out[0] = norm;
-        out[1] = !(max_norm > 0) ? (norm != norm ? norm : 1) : norm <= max_norm ? 1 : max_norm / norm;
-    }
+    if (threadIdx.x == 0) write_norm(sum, max_norm, out);
+}
+
+// few chunks: one workgroup, four chunks at a time, and no second launch (which costs more than what one compute unit takes for them)
+template <class G>
+__global__ __launch_bounds__(1024) void norm_one_kernel(const NormArgs a, double max_norm, double* out) {
+    double sum[4] = {};
+    for (int c = threadIdx.x >> 8; c < a.chunks; c += 4) add_chunk<G>(a, c, threadIdx.x & 255, sum);
+    const double all = block_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
+    if (threadIdx.x == 0) write_norm(all, max_norm, out);
 }
 
 int esize(int dt) { return dt == UDE_DT_F64 ? 8 : dt == UDE_DT_F32 ? 4 : 2; }
@@ -602,6 +618,18 @@ extern "C" int ude_grad_norm_dev(ude_ctx* c, int32_t dtype, int64_t nt, const vo
     if (!dev.ok) return fail(c, UDE_ERR_HIP, "grad_norm: device %d", c->device);
     NormArgs a{};
     int64_t sums = 0;
+    bool done = false;
+    auto run = [&](auto g, int64_t chunks) {
+        typedef decltype(g) G;
+        if (sums == 0 && chunks <= NORM_ONE && need <= 8 * chunks) {  // (they are all there are)
+            hipLaunchKernelGGL((norm_one_kernel<G>), dim3(1), dim3(1024), 0, c->stream, a, max_norm, out);
+            done = true;
+            return;
+        }
+        const unsigned blocks = (unsigned)(chunks < NORM_BLOCKS ? chunks : NORM_BLOCKS);
+        hipLaunchKernelGGL((norm_part_kernel<G>), dim3(blocks), dim3(256), 0, c->stream, a);
+        sums += blocks;
+    };
     const int rc = in_launches(
         nt, NORM_NT, NORM_CHUNK, a.first, [&](int64_t i) { return n[i]; },
         [&](int slot, int64_t i) { a.g[slot] = grads[i], a.n[slot] = n[i]; },
@@ -609,20 +637,18 @@ extern "C" int ude_grad_norm_dev(ude_ctx* c, int32_t dtype, int64_t nt, const vo
             a.nt = used;
             a.chunks = (int32_t)chunks;
             a.part = (double*)ws + sums;
-            const unsigned g = (unsigned)(chunks < NORM_BLOCKS ? chunks : NORM_BLOCKS);
-            sums += g;
             if (dtype == UDE_DT_F64)
-                hipLaunchKernelGGL((norm_part_kernel<DF64>), dim3(g), dim3(256), 0, c->stream, a);
+                run(DF64(), chunks);
             else if (dtype == UDE_DT_F32)
-                hipLaunchKernelGGL((norm_part_kernel<DF32>), dim3(g), dim3(256), 0, c->stream, a);
+                run(DF32(), chunks);
             else if (dtype == UDE_DT_F16)
-                hipLaunchKernelGGL((norm_part_kernel<DF16>), dim3(g), dim3(256), 0, c->stream, a);
+                run(DF16(), chunks);
             else
-                hipLaunchKernelGGL((norm_part_kernel<DBF16>), dim3(g), dim3(256), 0, c->stream, a);
+                run(DBF16(), chunks);
             HIPCHK(c, hipGetLastError());
             return (int)UDE_OK;
         });
-    if (rc) return rc;
+    if (rc || done) return rc;
     hipLaunchKernelGGL(norm_join_kernel, dim3(1), dim3(256), 0, c->stream, (const double*)ws, (int)sums, max_norm, out);
     HIPCHK(c, hipGetLastError());
     return UDE_OK;

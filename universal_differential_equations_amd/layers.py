@@ -9,26 +9,37 @@ columns (`vec(W)` of Flux / Lux: W = torch.empty(n_in, n_out).T), all three in t
 import ctypes as C
 
 from . import _lib
-from .sciml import Engine
+from .sciml import Engine, current_raw_stream
 
 
 def _order(name, w):
     """1: rows adjacent, 0: columns adjacent, None: either (a single row or column fits both)"""
-    rows, cols = w.shape
-    by_rows = w.stride(1) == 1 or cols == 1
-    by_cols = w.stride(0) == 1 or rows == 1
-    if by_rows and by_cols:
-        return None
-    if not by_rows and not by_cols:
+    (rows, cols), (r, c) = w.shape, w.stride()
+    by_rows = c == 1 or cols == 1
+    by_cols = r == 1 or rows == 1
+    if by_rows != by_cols:
+        return 1 if by_rows else 0
+    if not by_rows:
         raise ValueError("%s: one of its axes has to be contiguous, strides are %s" % (name, w.stride()))
-    return 1 if by_rows else 0
+    return None
 
 
 def _ld(w, order):
     """elements from one row (order 1) or column (order 0) to the next"""
-    rows, cols = w.shape
-    n, length, ld = (rows, cols, w.stride(0)) if order else (cols, rows, w.stride(1))
+    (rows, cols), (r, c) = w.shape, w.stride()
+    n, length, ld = (rows, cols, r) if order else (cols, rows, c)
     return ld if n > 1 else max(ld, length)
+
+
+_KINDS = {}
+
+
+def _kinds():
+    """torch dtype -> UDE_DT_* (torch is not imported before the first call)"""
+    if not _KINDS:
+        import torch
+        _KINDS.update({getattr(torch, k): _lib.DTYPE_CODE[k] for k in ("float32", "float16", "bfloat16")})
+    return _KINDS
 
 
 class _Block:
@@ -36,38 +47,36 @@ class _Block:
 
     def __init__(self, x, w_gate, w_up, w_down, act):
         import torch
-        ws = (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down))
-        if x.device.type != "cuda":
-            raise ValueError("gated_ffn: x is on %s, a CUDA tensor is needed (there is no CPU fallback)" % x.device)
-        if str(x.dtype)[6:] not in ("float32", "float16", "bfloat16"):
-            raise ValueError("gated_ffn: x is %s: float32, float16 and bfloat16 are supported" % x.dtype)
+        dev, dtype = x.device, x.dtype
+        if dev.type != "cuda":
+            raise ValueError("gated_ffn: x is on %s, a CUDA tensor is needed (there is no CPU fallback)" % dev)
+        code = _kinds().get(dtype)
+        if code is None:
+            raise ValueError("gated_ffn: x is %s: float32, float16 and bfloat16 are supported" % dtype)
         if x.dim() < 1:
             raise ValueError("gated_ffn: x has no axis of features")
-        for name, w in ws:
-            if w.device != x.device or w.dtype != x.dtype:
-                raise ValueError("gated_ffn: %s is %s on %s, x is %s on %s" % (name, w.dtype, w.device, x.dtype, x.device))
+        for name, w in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
+            if w.dtype != dtype or w.device != dev:
+                raise ValueError("gated_ffn: %s is %s on %s, x is %s on %s" % (name, w.dtype, w.device, dtype, dev))
             if w.dim() != 2:
                 raise ValueError("gated_ffn: %s has %d axes, 2 are needed" % (name, w.dim()))
         d, f, o = x.shape[-1], w_gate.shape[0], w_down.shape[0]
-        if tuple(w_gate.shape) != (f, d) or tuple(w_up.shape) != (f, d) or tuple(w_down.shape) != (o, f):
+        if w_gate.shape != (f, d) or w_up.shape != (f, d) or w_down.shape != (o, f):
             raise ValueError("gated_ffn: x (..., %d) with w_gate %s, w_up %s, w_down %s: (F, D), (F, D), (O, F) are needed"
                              % (d, tuple(w_gate.shape), tuple(w_up.shape), tuple(w_down.shape)))
-        if act not in _lib.GATE:
+        gate = _lib.GATE.get(act)
+        if gate is None:
             raise ValueError("gated_ffn: act %r, one of %s is needed" % (act, sorted(_lib.GATE)))
-        orders = {o_ for o_ in (_order(name, w) for name, w in ws) if o_ is not None}
+        orders = {_order("gated_ffn: w_gate", w_gate), _order("gated_ffn: w_up", w_up), _order("gated_ffn: w_down", w_down)} - {None}
         if len(orders) > 1:
-            raise ValueError("gated_ffn: the weights are held in different orders (strides %s)" % ", ".join(str(w.stride()) for _, w in ws))
+            raise ValueError("gated_ffn: the weights are held in different orders (strides %s)" % ", ".join(str(w.stride()) for w in (w_gate, w_up, w_down)))
         order = orders.pop() if orders else 1
-        self.torch, self.shape, self.act = torch, x.shape, act
-        self.x = _rows(x.reshape(-1, d))
+        self.torch, self.shape, self.device, self.dtype = torch, x.shape, dev, dtype
+        self.x = _rows(x if x.dim() == 2 else x.reshape(-1, d))
         self.w = (w_gate, w_up, w_down)
-        D = _lib.GatedFfnDesc()
-        D.dtype, D.act, D.w_order = _lib.DTYPE_CODE[str(x.dtype)[6:]], _lib.GATE[act], order
-        D.T, D.D, D.F, D.O = self.x.shape[0], d, f, o
-        D.ldx, D.ldy = max(self.x.stride(0), d), o
-        D.ldg, D.ldu, D.ldd = _ld(w_gate, order), _ld(w_up, order), _ld(w_down, order)
-        self.D = D
-        self.eng = Engine.get(x.device.index)
+        self.D = _lib.GatedFfnDesc(code, gate, order, 0, self.x.shape[0], d, f, o, max(self.x.stride(0), d), o,
+                                   _ld(w_gate, order), _ld(w_up, order), _ld(w_down, order))
+        self.eng = Engine.get(dev.index)
 
     def workspace(self, pullback):
         n = C.c_int64(0)
@@ -75,10 +84,10 @@ class _Block:
         if rc:
             raise _lib.UdeError(rc, "gated_ffn: sizes T = %d, D = %d, F = %d, O = %d" % (self.D.T, self.D.D, self.D.F, self.D.O))
         # (from torch's allocator on the current stream: a captured call gets memory of its graph, two calls never share one)
-        return self.torch.empty(max(n.value, 256), dtype=self.torch.uint8, device=self.x.device)
+        return self.torch.empty(max(n.value, 256), dtype=self.torch.uint8, device=self.device), n.value
 
     def bind(self):
-        self.eng.set_stream(self.torch.cuda.current_stream(self.x.device).cuda_stream)
+        self.eng.set_stream(current_raw_stream(self.device.index))
 
 
 def _rows(x):
@@ -95,15 +104,17 @@ def gated_ffn(x, w_gate, w_up, w_down, act="swish", save=False):
     sigmoid, swish, gelu_tanh or gelu_erf.  save=True returns (y, saved) for `gated_ffn_pullback`: `saved` holds references to x and the
     weights -- change them in place only after the pullback -- and Wg x, Wu x in Float32."""
     b = _Block(x, w_gate, w_up, w_down, act)
-    torch = b.torch
-    t, f, o = b.D.T, b.D.F, b.D.O
-    y = torch.empty((t, o), dtype=x.dtype, device=x.device)
-    b.gate = torch.empty((2, t, f), dtype=torch.float32, device=x.device) if save else None
-    ws = b.workspace(0)
+    torch, D = b.torch, b.D
+    t, f, o = D.T, D.F, D.O
+    y = torch.empty((t, o), dtype=b.dtype, device=b.device)
+    b.gate = torch.empty((2, t, f), dtype=torch.float32, device=b.device) if save else None
+    gate = b.gate.data_ptr() if save else None
+    ws, size = b.workspace(0)
     b.bind()
-    b.eng.check(b.eng.L.ude_gated_ffn_forward_dev(b.eng.h, C.byref(b.D), _p(b.x), _p(w_gate), _p(w_up), _p(w_down), _p(y),
-                                                  _p(b.gate), b.gate.data_ptr() + 4 * t * f if save else None, _p(ws), ws.numel()))
-    y = y.view(*b.shape[:-1], o)
+    b.eng.check(b.eng.L.ude_gated_ffn_forward_dev(b.eng.h, C.byref(D), b.x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
+                                                  y.data_ptr(), gate, gate + 4 * t * f if save else None, ws.data_ptr(), size))
+    if x.dim() != 2:
+        y = y.view(*b.shape[:-1], o)
     return (y, b) if save else y
 
 
@@ -112,27 +123,27 @@ def gated_ffn_pullback(saved, dy, need=("x", "w_gate", "w_up", "w_down")):
     The gradients of the weights are contiguous in the weights' order.  May be called again on the same `saved`."""
     b = saved
     torch = b.torch
-    if dy.device != b.x.device or dy.dtype != b.x.dtype or tuple(dy.shape) != tuple(b.shape[:-1]) + (b.D.O,):
+    if dy.dtype != b.dtype or dy.device != b.device or dy.shape[:-1] != b.shape[:-1] or dy.shape[-1] != b.D.O:
         raise ValueError("gated_ffn_pullback: dy is %s %s on %s, %s %s on %s is needed"
-                         % (dy.dtype, tuple(dy.shape), dy.device, b.x.dtype, tuple(b.shape[:-1]) + (b.D.O,), b.x.device))
+                         % (dy.dtype, tuple(dy.shape), dy.device, b.dtype, tuple(b.shape[:-1]) + (b.D.O,), b.device))
     unknown = set(need) - {"x", "w_gate", "w_up", "w_down"}
     if unknown:
         raise ValueError("gated_ffn_pullback: need has %s" % sorted(unknown))
-    dy = _rows(dy.reshape(-1, b.D.O))
+    dy = _rows(dy if dy.dim() == 2 else dy.reshape(-1, b.D.O))
     D = _lib.GatedFfnDesc.from_buffer_copy(b.D)
     D.ldy = max(dy.stride(0), D.O)
     t, f = D.T, D.F
-    dx = torch.empty((t, D.D), dtype=dy.dtype, device=dy.device) if "x" in need else None
+    dx = torch.empty((t, D.D), dtype=b.dtype, device=b.device) if "x" in need else None
     grads = []
     for name, w in zip(("w_gate", "w_up", "w_down"), b.w):
         rows, cols = w.shape
-        g = torch.empty((rows, cols) if D.w_order else (cols, rows), dtype=dy.dtype, device=dy.device) if name in need else None
+        g = torch.empty((rows, cols) if D.w_order else (cols, rows), dtype=b.dtype, device=b.device) if name in need else None
         grads.append(g if g is None or D.w_order else g.T)
-    ws = torch.empty(0, device=dy.device) if t == 0 else b.workspace(1)
+    ws, size = b.workspace(1)
+    gate = b.gate.data_ptr()
     b.bind()
-    b.eng.check(b.eng.L.ude_gated_ffn_backward_dev(b.eng.h, C.byref(D), _p(b.x), _p(b.w[0]), _p(b.w[1]), _p(b.w[2]),
-                                                   _p(b.gate), b.gate.data_ptr() + 4 * t * f, _p(dy), _p(dx), _p(grads[0]), _p(grads[1]), _p(grads[2]),
-                                                   _p(ws) or None, ws.numel()))
-    if dx is not None:
+    b.eng.check(b.eng.L.ude_gated_ffn_backward_dev(b.eng.h, C.byref(D), b.x.data_ptr(), *[w.data_ptr() for w in b.w], gate, gate + 4 * t * f, dy.data_ptr(),
+                                                   _p(dx), _p(grads[0]), _p(grads[1]), _p(grads[2]), ws.data_ptr(), size))
+    if dx is not None and dx.shape != b.shape:
         dx = dx.view(b.shape)
-    return (dx,) + tuple(grads)
+    return (dx, *grads)

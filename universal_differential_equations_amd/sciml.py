@@ -183,6 +183,14 @@ def _opts(alg, abstol=None, reltol=None, dtmax=None, dt=None, maxiters=None, sen
     return o
 
 
+def current_raw_stream(device):
+    """the hipStream_t of torch's current stream on a device, as torch.cuda.current_stream(device).cuda_stream gives it, without the two
+    microseconds that building a Stream object takes"""
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(device) if raw else torch.cuda.current_stream(device).cuda_stream
+
+
 def _is_torch(x):
     return type(x).__module__.startswith("torch")
 

@@ -17,7 +17,7 @@ from array import array
 import numpy as np
 
 from . import _lib
-from .sciml import Engine
+from .sciml import Engine, current_raw_stream
 
 
 def _xp(x):
@@ -70,9 +70,8 @@ def _device_list(what, tensors):
 
 
 def _bound_engine(dev):
-    import torch
     eng = Engine.get(dev.index)
-    eng.set_stream(torch.cuda.current_stream(dev).cuda_stream)
+    eng.set_stream(current_raw_stream(dev.index))
     return eng
 
 
