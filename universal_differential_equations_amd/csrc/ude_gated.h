@@ -122,7 +122,7 @@ struct Product {
     int64_t lda, ldb, ldc;
     int M, N;
     int vecA, vecB;  // 16-byte loads allowed: base and leading dimension aligned (gemm_any)
-    int vecC;        // stores of four consecutive columns allowed
+    int vecC;        // rows of C begin on a multiple of so many elements: 4, 2 or 1
 };
 struct Args {
     Product p[3];  // EPI_STORE: nprod of them side by side, or (nseg = 2) p[0] + p[1] into p[0].C; EPI_GATE: B of p[0] and p[1]
@@ -134,6 +134,7 @@ struct Args {
     float* part;
     int64_t room;  // bytes there
     float *gate, *up;     // EPI_GATE: stored if not NULL; EPI_PULL: read; leading dimension N
+    int vecG;             // ... whose rows begin on a multiple of so many elements
     void *dg, *du, *h;    // EPI_PULL: dg and du with leading dimension p[0].ldc, h with ldh
     int64_t ldh;
 };
@@ -156,23 +157,33 @@ static __device__ inline void load8(const E* p, int64_t left, bool row, int vec,
 }
 
 // What a kernel does with N times four consecutive columns n[].. of rows m[] (v: Wu's products for EPI_GATE)
+// Rows begin on a multiple of `vec` elements (4, 2 or 1); left = columns from here on
 template <class T>
-static __device__ inline void store4(typename T::E* to, const float* x, int left, bool vec) {
+static __device__ inline void store4(typename T::E* to, const float* x, int left, int vec) {
     typedef typename T::E E;
     typedef E E4 __attribute__((ext_vector_type(4)));
+    typedef E E2 __attribute__((ext_vector_type(2)));
     const E4 o = {T::from(x[0]), T::from(x[1]), T::from(x[2]), T::from(x[3])};
-    if (vec && left >= 4)
+    if (vec == 4 && left >= 4) {
         *(E4*)to = o;
-    else
+    } else if (vec >= 2 && left >= 4) {
+        ((E2*)to)[0] = E2{o[0], o[1]};
+        ((E2*)to)[1] = E2{o[2], o[3]};
+    } else {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
             if (q < left) to[q] = o[q];
+    }
 }
-static __device__ inline void load4(const float* p, float* o, int left, bool vec) {
-    if (vec && left >= 4) {
+static __device__ inline void load4(const float* p, float* o, int left, int vec) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    if (vec == 4 && left >= 4) {
         const f4 x = *(const f4*)p;
 #pragma unroll
         for (int q = 0; q < 4; ++q) o[q] = x[q];
+    } else if (vec >= 2 && left >= 4) {
+        const f2 x = ((const f2*)p)[0], y = ((const f2*)p)[1];
+        o[0] = x[0], o[1] = x[1], o[2] = y[0], o[3] = y[1];
     } else {
 #pragma unroll
         for (int q = 0; q < 4; ++q) o[q] = q < left ? p[q] : 0.f;
@@ -198,8 +209,8 @@ static __device__ inline void finish(const Args& a, const Product& p, const int*
                 store4<T>((E*)p.C + (int64_t)m[i] * p.ldc + n[i], h, p.N - n[i], p.vecC);
                 if (a.gate) {
                     const int64_t at = (int64_t)m[i] * p.N + n[i];
-                    store4<F32>(a.gate + at, (const float*)&c[i], p.N - n[i], p.vecC);
-                    store4<F32>(a.up + at, (const float*)&v[i], p.N - n[i], p.vecC);
+                    store4<F32>(a.gate + at, (const float*)&c[i], p.N - n[i], a.vecG);
+                    store4<F32>(a.up + at, (const float*)&v[i], p.N - n[i], a.vecG);
                 }
             }
     } else {
@@ -208,8 +219,8 @@ static __device__ inline void finish(const Args& a, const Product& p, const int*
         for (int i = 0; i < N; ++i) {
             const int64_t at = (int64_t)m[i] * p.N + n[i];
             const int left = m[i] < p.M ? p.N - n[i] : 0;
-            load4(a.gate + at, g + 4 * i, left, p.vecC);
-            load4(a.up + at, u + 4 * i, left, p.vecC);
+            load4(a.gate + at, g + 4 * i, left, a.vecG);
+            load4(a.up + at, u + 4 * i, left, a.vecG);
         }
         gate_acts<QUICK, 4 * N>(a.act, g, act, slope);
 #pragma unroll
@@ -446,14 +457,18 @@ static __device__ inline Place place(const Args& a, int t) {
     return {z, (gm0 + (t - group * GM * nn) % gsize) * tm + corner % 2 * BM, (t - group * GM * nn) / gsize * tn + corner / 2 * NT};
 }
 
-template <class T, int EPI, bool AK, bool BKc, int BM, int BN, int NWM, int NWN, int OCC>
+// STAGES: so many buffers of both operands, each step loaded that many steps ahead; 0: three of A and two of B, which is what 256 x 256 and two
+// workgroups of 128 x 128 leave room for.
+template <class T, int EPI, bool AK, bool BKc, int BM, int BN, int NWM, int NWN, int OCC, int STAGES>
 __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void gemm_tile(const Args a) {
     constexpr int NW = NWM * NWN, FM = BM / NWM / 16, FN = BN / NWN / 16, HALVES = EPI == EPI_GATE ? 2 : 1;
     constexpr int NT = BN / HALVES;  // output columns of a tile
     typedef Operand<T, AK, BM, NW, 1> OA;
     typedef Operand<T, BKc, BN, NW, HALVES> OB;
     constexpr int KS = OA::KS;
-    constexpr int BUFFERS = 2 * OB::BYTES + 3 * OA::BYTES;  // two of B, then three of A
+    constexpr bool DEEP = STAGES > 0;
+    constexpr int STAGE = OA::BYTES + OB::BYTES;  // DEEP: a step's A, then its B; otherwise two of B, then three of A
+    constexpr int BUFFERS = DEEP ? STAGES * STAGE : 2 * OB::BYTES + 3 * OA::BYTES;
     __shared__ __attribute__((aligned(1024))) char lds[BUFFERS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % NWM, wn = wave / NWM;
     int t = on_its_xcd((int)blockIdx.x, (int)gridDim.x);
@@ -491,10 +506,12 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
                 fa[half][r - FN] = read_a(r - FN, half, sa);
         }
     };
-    // Step n, whose first half is in registers, out of the buffers sa and sb; leaves the first half of step n + 1 there, starts the loads of
-    // B's step n + 2 and of A's step n + 3.  (The loads of a step take about as long to issue as half a step's products: A's third buffer
-    // lets the later half of them arrive a step later.)
-    auto body = [&](int sa, int sa1, int sb, int n, int last) {
+    // Step n, whose first half is in registers, out of the buffers sa and sb; leaves the first half of step n + 1 (in sa1, sb1) there, starts
+    // the loads of the steps that come to lie in sa and sb.  A load has one step less than it is ahead to arrive: about 0.4 microseconds out
+    // of L2, which is what a step of a small tile took with two buffers.  (Without DEEP the loads of a step take about as long to issue as
+    // half a step's products: A's third buffer lets the later half of them arrive a step later.)
+    constexpr int AHEAD_A = DEEP ? STAGES : 3, AHEAD_B = DEEP ? STAGES : 2, OUT = DEEP ? (STAGES - 2) * (OA::N + OB::N) : OA::N;
+    auto body = [&](int sa, int sa1, int sb, int sb1, int n, int last) {
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
             reads(i, 1, sa, sb);
@@ -502,11 +519,11 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
             for (int j = 0; j < FN; ++j) acc[i][j] = T::mfma(fb[0][j], fa[0][i], acc[i][j]);
             __builtin_amdgcn_sched_barrier(0);
         }
-        // step n + 1 has arrived but for what A's loads brought for n + 2, and nobody reads this step's buffers any more
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(OA::N) : "memory");
+        // step n + 1 has arrived (the loads behind it need not have), and nobody reads this step's buffers any more
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(OUT) : "memory");
         __builtin_amdgcn_sched_barrier(0);
         // (where no step is left to load, the last one is loaded again, into a buffer that is not read)
-        const int nb = n + 2 < last ? n + 2 : last, na = n + 3 < last ? n + 3 : last;
+        const int nb = n + AHEAD_B < last ? n + AHEAD_B : last, na = n + AHEAD_A < last ? n + AHEAD_A : last;
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
 #pragma unroll
@@ -515,13 +532,13 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
                     ob.piece(p, at + sb, wave, nb);
                 else
                     oa.piece(p - OB::N, at + sa, wave, na);
-            reads(i, 0, sa1, OB::BYTES - sb);
+            reads(i, 0, sa1, sb1);
 #pragma unroll
             for (int j = 0; j < FN; ++j) acc[i][j] = T::mfma(fb[1][j], fa[1][i], acc[i][j]);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    constexpr int A0 = 2 * OB::BYTES, A1 = A0 + OA::BYTES, A2 = A1 + OA::BYTES;
+    constexpr int A0 = DEEP ? 0 : 2 * OB::BYTES, A1 = A0 + OA::BYTES, A2 = A1 + OA::BYTES, B0 = DEEP ? OA::BYTES : 0;
     // Offsets within a run of steps stay below 2^31: a run of an "R" operand with long rows is shorter than K
     int64_t most = 1 << 22;
     if (!AK && (1 << 30) / (128 * q.lda) < most) most = (1 << 30) / (128 * q.lda);
@@ -547,31 +564,46 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
             const int left = (int)((kend - k0) / KS), full = left < run ? left : run, rest = left < run ? (int)((kend - k0) % KS) : 0;
             if (full) {
                 const int last = full - 1;
-                load_a(A0, 0), load_b(0, 0);
-                load_a(A1, 1 < last ? 1 : last), load_b(OB::BYTES, 1 < last ? 1 : last);
-                load_a(A2, 2 < last ? 2 : last);
-                asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * OA::N + OB::N) : "memory");
+                if constexpr (DEEP) {
 #pragma unroll
-                for (int j = 0; j < FN; ++j) fb[0][j] = read_b(j, 0, 0);
+                    for (int k = 0; k < STAGES; ++k) load_a(k * STAGE, k < last ? k : last), load_b(k * STAGE + B0, k < last ? k : last);
+                    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((STAGES - 1) * (OA::N + OB::N)) : "memory");
+                } else {
+                    load_a(A0, 0), load_b(0, 0);
+                    load_a(A1, 1 < last ? 1 : last), load_b(OB::BYTES, 1 < last ? 1 : last);
+                    load_a(A2, 2 < last ? 2 : last);
+                    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * OA::N + OB::N) : "memory");
+                }
+#pragma unroll
+                for (int j = 0; j < FN; ++j) fb[0][j] = read_b(j, 0, B0);
 #pragma unroll
                 for (int i = 0; i < FM; ++i) fa[0][i] = read_a(i, 0, A0);
-                int s0 = A0, s1 = A1, s2 = A2;
-                for (int n = 0; n < full; n += 2) {
-                    body(s0, s1, 0, n, last);
-                    if (n + 1 < full) body(s1, s2, OB::BYTES, n + 1, last);
-                    const int s = s0;
-                    s0 = s2, s2 = s1, s1 = s;
+                if constexpr (DEEP) {
+                    int here = 0;
+                    for (int n = 0; n < full; ++n) {
+                        const int next = here + STAGE < STAGES * STAGE ? here + STAGE : 0;
+                        body(here, next, here + B0, next + B0, n, last);
+                        here = next;
+                    }
+                } else {
+                    int s0 = A0, s1 = A1, s2 = A2;
+                    for (int n = 0; n < full; n += 2) {
+                        body(s0, s1, 0, OB::BYTES, n, last);
+                        if (n + 1 < full) body(s1, s2, OB::BYTES, 0, n + 1, last);
+                        const int s = s0;
+                        s0 = s2, s2 = s1, s1 = s;
+                    }
                 }
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             }
             if (rest) {
                 oa.tail(at + A0, wave, lane, full, rest, lds + A0);
-                ob.tail(at, wave, lane, full, rest, lds);
+                ob.tail(at + B0, wave, lane, full, rest, lds + B0);
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk) {
 #pragma unroll
-                    for (int j = 0; j < FN; ++j) fb[0][j] = read_b(j, kk, 0);
+                    for (int j = 0; j < FN; ++j) fb[0][j] = read_b(j, kk, B0);
 #pragma unroll
                     for (int i = 0; i < FM; ++i) fa[0][i] = read_a(i, kk, A0);
 #pragma unroll

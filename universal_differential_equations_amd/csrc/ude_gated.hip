@@ -44,8 +44,8 @@ int vec(const void* p, int64_t ld, int e) { return (uintptr_t)p % 16 == 0 && ld 
 // Tiles on the 256 compute units of an MI355X: microseconds that a step of 128 bytes of k takes with 1, 2, 3 workgroups on a compute unit, and
 // the start and epilogue of a round, as measured (kernel times over products of 64 x 512 x 1408 to 4096 x 4096 x 11264).
 //   256 x 256: the least that is read again: 4096 x 4096 x 11264 in 271 us = 1395 TFLOP/s; 256 x 128: 311 us; 128 x 128: 365 us.
-//   The smaller ones leave less of the last round idle; a step costs them 0.4 to 0.5 however little there is in it (barrier, LDS, the loads'
-//   way), so that 64 and 32 rows are for small products, and for Float32, whose matrix instructions (1/16 of the 16-bit rate) bound it with
+//   The smaller ones leave less of the last round idle, but a step costs them 0.25 to 0.5 however little there is in it (LDS, barrier, the
+//   loads' way: 64 x 64 takes 0.25 with its loads four steps ahead, 0.41 with two), so that they are for small products, and for Float32, whose matrix instructions (1/16 of the 16-bit rate) bound it with
 //   any tile.
 // EPI_GATE writes ten bytes an element at the end, EPI_PULL reads eight and writes six.  Where tiles are few and K is long, K is cut into
 // parts whose sums go through memory (3 TB/s) and one more launch.
@@ -54,7 +54,7 @@ constexpr int64_t MOST_PART_BYTES = (int64_t)2 * CUS * 128 * 128 * 4;
 enum { T256 = 0, T256x128 = 1, T128 = 2, T64 = 3, T32 = 4, TILES = 5 };
 struct Tile {
     int bm, bn, bn_gate;             // EPI_GATE: of which half are output columns
-    int slots, slots_gate;           // workgroups of a compute unit
+    int slots, slots32;              // workgroups of a compute unit, 16-bit kinds and Float32
     double step[3], gate[3];         // 16-bit kinds; EPI_GATE's where its tile is another
     double step32[3], gate32[3];     // Float32 (0: there is none)
     double end[3];                   // EPI_STORE, EPI_GATE, EPI_PULL
@@ -63,7 +63,7 @@ constexpr Tile TILE[TILES] = {
     {256, 256, 256, 1, 1, {1.48}, {1.48}, {}, {}, {6, 17, 42}},
     {256, 128, 128, 1, 1, {0.87}, {0.87}, {}, {}, {5, 10, 25}},
     {128, 128, 128, 2, 2, {0.48, 1.02}, {0.48, 1.02}, {1.95, 3.8}, {1.95, 3.8}, {6, 9, 17}},
-    {64, 64, 128, 3, 2, {0.41, 0.43, 0.62}, {0.45, 0.66}, {0.54, 1.08, 1.6}, {1.08, 2.1}, {4, 6, 7}},
+    {64, 64, 128, 2, 3, {0.25, 0.43}, {0.40, 0.64}, {0.54, 1.08, 1.6}, {1.08, 2.1, 3.2}, {4, 6, 7}},
     {32, 128, 128, 3, 3, {0.46, 0.50, 0.65}, {0.46, 0.50, 0.65}, {0.55, 1.1, 1.65}, {0.55, 1.1, 1.65}, {4, 5, 7}}};
 struct Plan {
     int which, split;  // tile; parts of K
@@ -76,11 +76,11 @@ int64_t tiles_of(const Args& a, int epi, int which) {
     for (int i = 0; i < a.nprod; ++i) n += (int64_t)((a.p[i].M + bm - 1) / bm) * ((a.p[i].N + bn - 1) / bn);
     return n;
 }
-int slots_of(int which, int epi) { return epi == EPI_GATE ? TILE[which].slots_gate : TILE[which].slots; }
+int slots_of(int which, int es) { return es == 4 ? TILE[which].slots32 : TILE[which].slots; }
 double tiles_cost(int which, int epi, int es, int64_t n, double steps) {
     const Tile& t = TILE[which];
     const double* c = epi == EPI_GATE ? (es == 4 ? t.gate32 : t.gate) : (es == 4 ? t.step32 : t.step);
-    const int slots = slots_of(which, epi);
+    const int slots = slots_of(which, es);
     const int64_t whole = n / (slots * CUS), rest = (n % (slots * CUS) + CUS - 1) / CUS;
     return whole * (steps * c[slots - 1] + t.end[epi]) + (rest ? steps * c[rest - 1] + t.end[epi] : 0);
 }
@@ -89,7 +89,7 @@ int64_t part_size(int which, int epi) { return (int64_t)TILE[which].bm * (epi ==
 double cut(int which, int epi, int es, int64_t n, int total, int64_t room, int* parts) {
     double least = tiles_cost(which, epi, es, n, total);
     *parts = 1;
-    for (int s = 2; s * n <= slots_of(which, epi) * CUS && s * n * part_size(which, epi) <= room && s * 2 <= total; ++s) {
+    for (int s = 2; s * n <= slots_of(which, es) * CUS && s * n * part_size(which, epi) <= room && s * 2 <= total; ++s) {
         const double c = tiles_cost(which, epi, es, n * s, (total + s - 1) / s) + n * s * part_size(which, epi) * (2 / 3e6) + 6;
         if (c < least) least = c, *parts = s;
     }
@@ -138,23 +138,23 @@ template <class T, int EPI, bool AK, bool BKc>
 int launch3(ude_ctx* c, Args a, bool tile) {
     const Plan p = plan(a, EPI, AK, sizeof(typename T::E), a.room);
     if (tile && p.big * p.split < 1 << 22 && p.all < 1 << 22) {
-        constexpr bool GATE = EPI == EPI_GATE;
+        constexpr bool GATE = EPI == EPI_GATE, HALF = sizeof(typename T::E) == 2;
         a.split = p.split;
         const dim3 grid((unsigned)(p.big * p.split)), block(256);
         auto go = [&](auto kernel, dim3 g) { hipLaunchKernelGGL(kernel, g, block, 0, c->stream, a); };
-        if constexpr (sizeof(typename T::E) == 2) {
-            if (p.which == T256) go(gemm_tile<T, EPI, AK, BKc, 256, 256, 2, 2, 1>, grid);
-            if (p.which == T256x128) go(gemm_tile<T, EPI, AK, BKc, 256, 128, 2, 2, 1>, grid);
+        if constexpr (HALF) {
+            if (p.which == T256) go(gemm_tile<T, EPI, AK, BKc, 256, 256, 2, 2, 1, 0>, grid);
+            if (p.which == T256x128) go(gemm_tile<T, EPI, AK, BKc, 256, 128, 2, 2, 1, 0>, grid);
         }
-        if (p.which == T128) go(gemm_tile<T, EPI, AK, BKc, 128, 128, 2, 2, 2>, grid);
-        if (p.which == T64) go(gemm_tile<T, EPI, AK, BKc, 64, GATE ? 128 : 64, 2, 2, GATE ? 2 : 3>, grid);
+        if (p.which == T128) go(gemm_tile<T, EPI, AK, BKc, 128, 128, 2, 2, 2, 0>, grid);
+        if (p.which == T64) go(gemm_tile<T, EPI, AK, BKc, 64, GATE ? 128 : 64, 2, 2, HALF || GATE ? 2 : 3, HALF ? (GATE ? 3 : 4) : 0>, grid);
         if constexpr (AK)
-            if (p.which == T32) go(gemm_tile<T, EPI, AK, BKc, 32, 128, 1, 4, 3>, grid);
+            if (p.which == T32) go(gemm_tile<T, EPI, AK, BKc, 32, 128, 1, 4, 3, 0>, grid);
         HIPCHK(c, hipGetLastError());
         if (p.quarters) {
             const unsigned rest = (unsigned)(4 * (p.all - p.big));
             a.first = (int)p.big, a.quarters = 1, a.split = p.quarters;
-            go(gemm_tile<T, EPI, AK, BKc, 128, 128, 2, 2, 2>, dim3(rest * p.quarters));
+            go(gemm_tile<T, EPI, AK, BKc, 128, 128, 2, 2, 2, 0>, dim3(rest * p.quarters));
             HIPCHK(c, hipGetLastError());
             if (p.quarters > 1) go(join_parts<T, EPI, 128, 128, 2, 2>, dim3(rest, 4));
             HIPCHK(c, hipGetLastError());
@@ -185,6 +185,11 @@ int launch2(ude_ctx* c, const Args& a, bool ak, bool bk, bool tile) {
         if (!ak) return bk ? fail(c, UDE_ERR_INVALID, "gated_ffn: operand orders") : launch3<T, EPI, false, false>(c, a, tile);
     return bk ? launch3<T, EPI, true, true>(c, a, tile) : launch3<T, EPI, true, false>(c, a, tile);
 }
+// rows begin on a multiple of so many elements
+int begins(const void* p, int64_t ld, int e) {
+    return (uintptr_t)p % (4 * e) == 0 && ld % 4 == 0 ? 4 : (uintptr_t)p % (2 * e) == 0 && ld % 2 == 0 ? 2 : 1;
+}
+
 // ak, bk: consecutive k are adjacent
 template <int EPI>
 int launch(ude_ctx* c, int dtype, Args a, bool ak, bool bk) {
@@ -194,11 +199,11 @@ int launch(ude_ctx* c, int dtype, Args a, bool ak, bool bk) {
     for (int i = 0; i < used; ++i) {
         Product& p = a.p[i];
         p.vecA = vec(p.A, p.lda, e), p.vecB = vec(p.B, p.ldb, e);
-        p.vecC = (uintptr_t)p.C % (4 * e) == 0 && p.ldc % 4 == 0;
-        // gate and up are rows of N floats; dg, du, h lie in the workspace, rows of a multiple of 8
-        if (EPI != EPI_STORE && a.gate && (p.N % 4 || (uintptr_t)a.gate % 16 || (uintptr_t)a.up % 16)) p.vecC = 0;
+        p.vecC = begins(p.C, p.ldc, e);
         tile = tile && tileable(p.A, p.lda, e) && tileable(p.B, p.ldb, e);
     }
+    const int g = begins(a.gate, a.p[0].N, 4), u = begins(a.up, a.p[0].N, 4);
+    a.vecG = g < u ? g : u;
     if (dtype == UDE_DT_F32) return launch2<F32, EPI>(c, a, ak, bk, tile);
     if (dtype == UDE_DT_F16) return launch2<F16, EPI>(c, a, ak, bk, tile);
     return launch2<BF16, EPI>(c, a, ak, bk, tile);
