@@ -130,7 +130,7 @@ struct Args {
     int act;
     // gemm_tile: the tiles from `first` on; quarters: each workgroup a quarter of a 256 x 256 tile; split > 1: each a part of K, the
     // sums of tile t and part s go to part[(t * split + s) * tile size] and join_parts adds them up
-    int first, quarters, split;
+    int first, quarters, split, tiles;  // tiles: of this launch
     float* part;
     int64_t room;  // bytes there
     float *gate, *up;     // EPI_GATE: stored if not NULL; EPI_PULL: read; leading dimension N
@@ -138,6 +138,15 @@ struct Args {
     void *dg, *du, *h;    // EPI_PULL: dg and du with leading dimension p[0].ldc, h with ldh
     int64_t ldh;
 };
+
+// Kernel arguments lie in memory that the scalar cache has to fetch line by line, about a microsecond each when a kernel begins; read where
+// they are first used, one after the other, they cost a small product more than its arithmetic.  This asks for all lines at once.
+template <class A>
+static __device__ inline void touch(const A& a) {
+    const int* p = (const int*)&a;
+    static_assert(sizeof(A) > 64 * 4 && sizeof(A) <= 64 * 6, "one word of each line");
+    asm volatile("" ::"s"(p[0]), "s"(p[16]), "s"(p[32]), "s"(p[48]), "s"(p[64]), "s"(p[sizeof(A) / 4 - 1]));
+}
 
 // 8 consecutive elements along the stored axis of a tile; elements outside are zero
 template <class E>
@@ -387,10 +396,18 @@ struct Operand {
             }
         }
     }
-    // piece i of the whole step n to LDS at `at`
-    __device__ inline void piece(int i, unsigned at, int wave, int n) {
+    // the pieces of the whole step n; on = false: zeros, without a trip to memory
+    unsigned from[HALVES];
+    int size[HALVES];
+    __device__ inline void aim(int n, bool on) {
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) from[h] = on ? n * step[h] : 0, size[h] = on ? rec[h][2] : 0;
+    }
+    __device__ inline void piece(int i, unsigned at, int wave) {
         const int h = i / (N / HALVES);
-        to_lds(at + (i * NW + wave) * 1024, off[i], rec[h], n * step[h]);
+        i4 r = rec[h];
+        r[2] = size[h];
+        to_lds(at + (i * NW + wave) * 1024, off[i], r, from[h]);
     }
     // a last step of kleft < KS k, `n` steps behind k0; where it ends inside 16 bytes, a "K" operand goes element by element
     __device__ inline void tail(unsigned at, int wave, int lane, int n, int kleft, char* lds) {
@@ -470,10 +487,11 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
     constexpr int STAGE = OA::BYTES + OB::BYTES;  // DEEP: a step's A, then its B; otherwise two of B, then three of A
     constexpr int BUFFERS = DEEP ? STAGES * STAGE : 2 * OB::BYTES + 3 * OA::BYTES;
     __shared__ __attribute__((aligned(1024))) char lds[BUFFERS];
+    touch(a);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % NWM, wn = wave / NWM;
-    int t = on_its_xcd((int)blockIdx.x, (int)gridDim.x);
-    const int tiles = (int)gridDim.x / a.split, part = t / tiles;
-    const Place at_tile = place<BM, BN, HALVES>(a, t % tiles);
+    int t = on_its_xcd((int)blockIdx.x, a.tiles * a.split);
+    const int tiles = a.tiles, part = a.split > 1 ? t / tiles : 0;
+    const Place at_tile = place<BM, BN, HALVES>(a, a.split > 1 ? t % tiles : t);
     const Product& q = a.p[at_tile.z];
     const int z = at_tile.z, m0 = at_tile.m0, n0 = at_tile.n0;
     if (m0 >= q.M || n0 >= q.N) return;
@@ -487,13 +505,16 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
     auto read_b = [&](int j, int kk, int stage) {
         return OB::fragment(lds + stage, HALVES == 2 ? (j / (FN / 2)) * NT + wn * (NT / NWN) + (j % (FN / 2)) * 16 : wn * (BN / NWN) + j * 16, kk, lane);
     };
-    auto load_a = [&](int stage, int n) {
+    // (behind the last step: zeros, into buffers that are not read, so that the number of loads on their way is always the same)
+    auto load_a = [&](int stage, int n, int last) {
+        oa.aim(n, n <= last);
 #pragma unroll
-        for (int i = 0; i < OA::N; ++i) oa.piece(i, at + stage, wave, n);
+        for (int i = 0; i < OA::N; ++i) oa.piece(i, at + stage, wave);
     };
-    auto load_b = [&](int stage, int n) {
+    auto load_b = [&](int stage, int n, int last) {
+        ob.aim(n, n <= last);
 #pragma unroll
-        for (int i = 0; i < OB::N; ++i) ob.piece(i, at + stage, wave, n);
+        for (int i = 0; i < OB::N; ++i) ob.piece(i, at + stage, wave);
     };
     // rows of products are the grain that reads and loads are dealt out over; the compiler keeps the order of the grains
     auto reads = [&](int i, int half, int sa, int sb) {
@@ -519,19 +540,19 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
             for (int j = 0; j < FN; ++j) acc[i][j] = T::mfma(fb[0][j], fa[0][i], acc[i][j]);
             __builtin_amdgcn_sched_barrier(0);
         }
+        oa.aim(n + AHEAD_A, n + AHEAD_A <= last), ob.aim(n + AHEAD_B, n + AHEAD_B <= last);
+        __builtin_amdgcn_sched_barrier(0);
         // step n + 1 has arrived (the loads behind it need not have), and nobody reads this step's buffers any more
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(OUT) : "memory");
         __builtin_amdgcn_sched_barrier(0);
-        // (where no step is left to load, the last one is loaded again, into a buffer that is not read)
-        const int nb = n + AHEAD_B < last ? n + AHEAD_B : last, na = n + AHEAD_A < last ? n + AHEAD_A : last;
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
 #pragma unroll
             for (int p = i * (OA::N + OB::N) / FM; p < (i + 1) * (OA::N + OB::N) / FM; ++p)
                 if (p < OB::N)
-                    ob.piece(p, at + sb, wave, nb);
+                    ob.piece(p, at + sb, wave);
                 else
-                    oa.piece(p - OB::N, at + sa, wave, na);
+                    oa.piece(p - OB::N, at + sa, wave);
             reads(i, 0, sa1, sb1);
 #pragma unroll
             for (int j = 0; j < FN; ++j) acc[i][j] = T::mfma(fb[1][j], fa[1][i], acc[i][j]);
@@ -566,12 +587,12 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
                 const int last = full - 1;
                 if constexpr (DEEP) {
 #pragma unroll
-                    for (int k = 0; k < STAGES; ++k) load_a(k * STAGE, k < last ? k : last), load_b(k * STAGE + B0, k < last ? k : last);
+                    for (int k = 0; k < STAGES; ++k) load_a(k * STAGE, k, last), load_b(k * STAGE + B0, k, last);
                     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((STAGES - 1) * (OA::N + OB::N)) : "memory");
                 } else {
-                    load_a(A0, 0), load_b(0, 0);
-                    load_a(A1, 1 < last ? 1 : last), load_b(OB::BYTES, 1 < last ? 1 : last);
-                    load_a(A2, 2 < last ? 2 : last);
+                    load_a(A0, 0, last), load_b(0, 0, last);
+                    load_a(A1, 1, last), load_b(OB::BYTES, 1, last);
+                    load_a(A2, 2, last);
                     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * OA::N + OB::N) : "memory");
                 }
 #pragma unroll
@@ -661,12 +682,13 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
 template <class T, int EPI, int BM, int BN, int NWM, int NWN>
 __global__ __launch_bounds__(64 * NWM * NWN) void join_parts(const Args a) {
     constexpr int NW = NWM * NWN, FM = BM / NWM / 16, FN = BN / NWN / 16, HALVES = EPI == EPI_GATE ? 2 : 1, NT = BN / HALVES;
+    touch(a);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % NWM, wn = wave / NWM, i = blockIdx.y;
     const Place at = place<BM, BN, HALVES>(a, (int)blockIdx.x);
     const Product& q = a.p[at.z];
     const f4* from = (const f4*)a.part + (((int64_t)blockIdx.x * a.split) * NW + wave) * FM * FN * 64 + i * FN * 64 + lane;
     f4 sum[FN] = {};
-#pragma unroll 4
+#pragma unroll 8
     for (int s = 0; s < a.split; ++s)
 #pragma unroll
         for (int j = 0; j < FN; ++j) sum[j] += from[((int64_t)s * NW * FM * FN + j) * 64];

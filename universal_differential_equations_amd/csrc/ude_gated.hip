@@ -60,11 +60,11 @@ struct Tile {
     double end[3];                   // EPI_STORE, EPI_GATE, EPI_PULL
 };
 constexpr Tile TILE[TILES] = {
-    {256, 256, 256, 1, 1, {1.48}, {1.48}, {}, {}, {6, 17, 42}},
-    {256, 128, 128, 1, 1, {0.87}, {0.87}, {}, {}, {5, 10, 25}},
-    {128, 128, 128, 2, 2, {0.48, 1.02}, {0.48, 1.02}, {1.95, 3.8}, {1.95, 3.8}, {6, 9, 17}},
-    {64, 64, 128, 2, 3, {0.25, 0.43}, {0.40, 0.64}, {0.54, 1.08, 1.6}, {1.08, 2.1, 3.2}, {4, 6, 7}},
-    {32, 128, 128, 3, 3, {0.46, 0.50, 0.65}, {0.46, 0.50, 0.65}, {0.55, 1.1, 1.65}, {0.55, 1.1, 1.65}, {4, 5, 7}}};
+    {256, 256, 256, 1, 1, {1.46}, {1.46}, {}, {}, {12, 20, 45}},
+    {256, 128, 128, 1, 1, {0.85}, {0.85}, {}, {}, {9, 13, 28}},
+    {128, 128, 128, 2, 2, {0.48, 1.02}, {0.48, 1.02}, {1.95, 3.8}, {1.95, 3.8}, {7, 9, 17}},
+    {64, 64, 128, 2, 3, {0.25, 0.43}, {0.40, 0.64}, {0.54, 1.08, 1.6}, {1.08, 2.1, 3.2}, {5, 6, 7}},
+    {32, 128, 128, 3, 3, {0.46, 0.50, 0.65}, {0.46, 0.50, 0.65}, {0.55, 1.1, 1.65}, {0.55, 1.1, 1.65}, {5, 6, 7}}};
 struct Plan {
     int which, split;  // tile; parts of K
     int quarters;      // T256: whole rounds of them, the rest as quarters, cut into so many parts of K (0: no such rest)
@@ -139,7 +139,7 @@ int launch3(ude_ctx* c, Args a, bool tile) {
     const Plan p = plan(a, EPI, AK, sizeof(typename T::E), a.room);
     if (tile && p.big * p.split < 1 << 22 && p.all < 1 << 22) {
         constexpr bool GATE = EPI == EPI_GATE, HALF = sizeof(typename T::E) == 2;
-        a.split = p.split;
+        a.split = p.split, a.tiles = (int)p.big;
         const dim3 grid((unsigned)(p.big * p.split)), block(256);
         auto go = [&](auto kernel, dim3 g) { hipLaunchKernelGGL(kernel, g, block, 0, c->stream, a); };
         if constexpr (HALF) {
@@ -153,7 +153,7 @@ int launch3(ude_ctx* c, Args a, bool tile) {
         HIPCHK(c, hipGetLastError());
         if (p.quarters) {
             const unsigned rest = (unsigned)(4 * (p.all - p.big));
-            a.first = (int)p.big, a.quarters = 1, a.split = p.quarters;
+            a.first = (int)p.big, a.quarters = 1, a.split = p.quarters, a.tiles = (int)rest;
             go(gemm_tile<T, EPI, AK, BKc, 128, 128, 2, 2, 2, 0>, dim3(rest * p.quarters));
             HIPCHK(c, hipGetLastError());
             if (p.quarters > 1) go(join_parts<T, EPI, 128, 128, 2, 2>, dim3(rest, 4));
