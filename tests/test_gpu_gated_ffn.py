@@ -144,6 +144,23 @@ def test_rows_are_independent_and_non_finite_rows_stay_alone():
     assert torch.equal(z[keep], y[keep]) and not torch.isfinite(z[3]).any() and not torch.isfinite(z[69]).all()
 
 
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+@pytest.mark.parametrize("act", sorted(R.ACTS))
+def test_far_gates(act, kind):
+    """gates of any size: act and its derivative are finite (0 or 1 or g), so that u = 0 gives dg = 0"""
+    import universal_differential_equations_amd as U
+    most = 6e4 if kind == torch.float16 else 1e30
+    x = torch.tensor([[most], [-most], [200.0], [-200.0], [0.0], [1e-4]], dtype=kind, device="cuda")
+    one, zero = torch.ones(1, 1, dtype=kind, device="cuda"), torch.zeros(1, 1, dtype=kind, device="cuda")
+    y, saved = U.gated_ffn(x, one, zero, one, act=act, save=True)
+    dx, dwg, dwu, dwd = U.gated_ffn_pullback(saved, torch.ones_like(x))
+    assert not y.any() and not dwg.any() and not dwd.any() and not dx.any()
+    act64 = R.ACTS[act][0](x.double())
+    assert torch.isfinite(saved.gate).all() and torch.isfinite(act64).all()
+    y, saved = U.gated_ffn(x[2:], one, one, one, act=act, save=True)
+    assert torch.isfinite(y).all() and all(torch.isfinite(t).all() for t in U.gated_ffn_pullback(saved, torch.ones_like(y))) or kind == torch.float16
+
+
 def test_no_samples_and_partial_pullbacks():
     import universal_differential_equations_amd as U
     x, wg, wu, wd, dy = made(0, 24, 16, 40, torch.float16, False)
@@ -175,6 +192,36 @@ def test_output_rows_with_gaps_are_left_alone():
         assert bool((y[:, O:] == 7).all()) and bool((y[T] == 7).all())
         assert R.within(y[:T, :O], R.gated(x, wg, wu, wd, "swish")["y"]) <= 1
         assert _lib.GATE["swish"] == b.D.act
+
+
+def test_refusals():
+    import universal_differential_equations_amd as U
+    x, wg, wu, wd, dy = made(8, 24, 16, 40, torch.float16, True)
+    for bad in ((x.double(), wg, wu, wd), (x.float(), wg, wu, wd), (x, wg.cpu(), wu, wd), (x, wg[:8], wu, wd), (x, wg, wu[:, :8], wd), (x, wg, wu, wd.T.contiguous()),
+                (x[:, :23], wg, wu, wd), (x, wg, wu, wd[:, ::2]), (x, wg.T.contiguous().T, wu, wd), (x, wg[0], wu, wd), (x[:, :0], wg[:, :0], wu[:, :0], wd)):
+        with pytest.raises(ValueError):
+            U.gated_ffn(*bad)
+    with pytest.raises(ValueError):
+        U.gated_ffn(x, wg, wu, wd, act="softmax")
+    _, saved = U.gated_ffn(x, wg, wu, wd, save=True)
+    for bad in (dy.float(), dy[:4], dy[:, :39], dy.cpu()):
+        with pytest.raises(ValueError):
+            U.gated_ffn_pullback(saved, bad)
+    with pytest.raises(ValueError):
+        U.gated_ffn_pullback(saved, dy, need=("w",))
+
+
+def test_workspace_is_checked():
+    """too small a workspace, or one off its alignment, is refused before anything is launched"""
+    from universal_differential_equations_amd.layers import _Block
+    x, wg, wu, wd, _ = made(64, 512, 1408, 512, torch.bfloat16, True)
+    b = _Block(x, wg, wu, wd, "swish")
+    ws, size = b.workspace(0)
+    y = torch.full((64, 512), 7.0, dtype=torch.bfloat16, device="cuda")
+    b.bind()
+    for at, n in ((ws.data_ptr(), size - 1), (ws.data_ptr() + 16, size), (None, size)):
+        assert b.eng.L.ude_gated_ffn_forward_dev(b.eng.h, C.byref(b.D), *(t.data_ptr() for t in (x, wg, wu, wd, y)), None, None, at, n) == -1
+    assert bool((y == 7).all())
 
 
 def test_streams_and_graphs():

@@ -70,7 +70,7 @@ static __device__ inline float gate_act(float g, float* slope) {
         return e;
     } else if constexpr (ACT == UDE_GATE_RELU) {
         *slope = g > 0.f ? 1.f : 0.f;
-        return g > 0.f ? g : g * 0.f;  // (NaN stays NaN)
+        return g > 0.f ? g : g == g ? 0.f : g;  // (NaN stays NaN)
     } else if constexpr (ACT == UDE_GATE_SIGMOID) {
         const float s = sigmoid<QUICK>(g);
         *slope = s * (1.f - s);
@@ -81,8 +81,9 @@ static __device__ inline float gate_act(float g, float* slope) {
         return g * s;
     } else if constexpr (ACT == UDE_GATE_GELU_TANH) {
         const float c = 1.5957691216057308f, q = 0.044715f;  // 2 sqrt(2 / pi)
-        const float s = sigmoid<QUICK>(c * (g + q * g * g * g));
-        *slope = s + g * s * (1.f - s) * c * (1.f + 3.f * q * g * g);
+        const float x = fabsf(g) > 100.f ? copysignf(100.f, g) : g;  // (s is 0 or 1 there, and the cube would overflow)
+        const float s = sigmoid<QUICK>(c * (x + q * x * x * x));
+        *slope = s + x * s * (1.f - s) * c * (1.f + 3.f * q * x * x);
         return g * s;
     } else if constexpr (ACT == UDE_GATE_GELU_ERF) {
         const float p = 0.5f * erfcf(g * -0.7071067811865476f), x = -0.5f * g * g;

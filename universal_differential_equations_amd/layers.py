@@ -64,6 +64,8 @@ class _Block:
         if w_gate.shape != (f, d) or w_up.shape != (f, d) or w_down.shape != (o, f):
             raise ValueError("gated_ffn: x (..., %d) with w_gate %s, w_up %s, w_down %s: (F, D), (F, D), (O, F) are needed"
                              % (d, tuple(w_gate.shape), tuple(w_up.shape), tuple(w_down.shape)))
+        if min(d, f, o) < 1:
+            raise ValueError("gated_ffn: D = %d, F = %d, O = %d" % (d, f, o))
         gate = _lib.GATE.get(act)
         if gate is None:
             raise ValueError("gated_ffn: act %r, one of %s is needed" % (act, sorted(_lib.GATE)))
@@ -102,7 +104,8 @@ def _p(t):
 def gated_ffn(x, w_gate, w_up, w_down, act="swish", save=False):
     """y = Wd (act(Wg x) .* (Wu x)) for every row of x (..., D); w_gate, w_up: (F, D), w_down: (O, F).  act: identity, tanh, rbf, relu,
     sigmoid, swish, gelu_tanh or gelu_erf.  save=True returns (y, saved) for `gated_ffn_pullback`: `saved` holds references to x and the
-    weights -- change them in place only after the pullback -- and Wg x, Wu x in Float32."""
+    weights -- change them in place only after the pullback -- and Wg x, Wu x in Float32.  No autograd graph is recorded: the pullback is the
+    gradient.  Rounding: sums and act in Float32; act(..) .* (..) is rounded to x's dtype once, where it enters the last product."""
     b = _Block(x, w_gate, w_up, w_down, act)
     torch, D = b.torch, b.D
     t, f, o = D.T, D.F, D.O

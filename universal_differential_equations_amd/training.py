@@ -120,10 +120,6 @@ class AdamW:
         for i, p in enumerate(self.params):
             if not p.is_contiguous():
                 raise ValueError("AdamW: parameter %d is not contiguous (strides %s)" % (i, p.stride()))
-        used = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size(), i) for i, p in enumerate(self.params) if p.numel())
-        for (_, end, i), (start, _, j) in zip(used, used[1:]):
-            if start < end:
-                raise ValueError("AdamW: parameters %d and %d share memory" % (min(i, j), max(i, j)))
         n = len(self.params)
         decay = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
         if len(decay) != n:
@@ -134,6 +130,11 @@ class AdamW:
         if state is not None and len(state) != n:
             raise ValueError("AdamW: state of %d tensors for %d parameters" % (len(state), n))
         self._state = [self._make_state(i, master, None if state is None else state[i]) for i in range(n)]
+        used = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), i) for i, p in enumerate(self.params)
+                      for t in (p, *self._state[i].values()) if t.numel())
+        for (_, end, i), (start, _, j) in zip(used, used[1:]):
+            if start < end:
+                raise ValueError("AdamW: parameters %d and %d, or their states, share memory" % (min(i, j), max(i, j)))
         self._table = (_lib.AdamwTensor * n)()
         self._columns = np.frombuffer(self._table, dtype=np.int64).reshape(n, -1)   # the same memory; column 0: param, 1: grad, 7: n
         self._live = [0] * n
@@ -254,7 +255,7 @@ def adamw(loss_grad, theta, eta=0.001, beta=(0.9, 0.999), decay=0.01, maxiters=2
     it is larger.  theta: numpy, or a torch tensor; a CUDA tensor is updated by the fused step and stays on the device."""
     xp = _xp(theta)
     cuda = xp is not np and theta.is_cuda
-    theta = theta.clone() if xp is not np else np.array(theta, dtype=np.float64)
+    theta = theta.detach().clone(memory_format=xp.contiguous_format) if xp is not np else np.array(theta, dtype=np.float64)
     opt = AdamW([theta], eta=eta, beta=beta, eps=eps, weight_decay=decay) if cuda else None
     m, v = (None, None) if cuda else (xp.zeros_like(theta), xp.zeros_like(theta))
     losses, last = [], theta
