@@ -129,9 +129,9 @@ struct Args {
     Product p[3];  // EPI_STORE: nprod of them side by side, or (nseg = 2) p[0] + p[1] into p[0].C; EPI_GATE: B of p[0] and p[1]
     int K, nprod, nseg;
     int act;
-    // gemm_tile: the tiles from `first` on; quarters: each workgroup a quarter of a 256 x 256 tile; split > 1: each a part of K, the
-    // sums of tile t and part s go to part[(t * split + s) * tile size] and join_parts adds them up
-    int first, quarters, split, tiles;  // tiles: of this launch
+    // gemm_tile: the tiles from `first` on; tm, tn (not 0): a piece of such a larger tile each, in the order of those; split > 1: each a part
+    // of K, the sums of tile t and part s go to part[(t * split + s) * tile size] and join_parts adds them up
+    int first, tm, tn, split, tiles;  // tiles: of this launch
     float* part;
     int64_t room;  // bytes there
     float *gate, *up;     // EPI_GATE: stored if not NULL; EPI_PULL: read; leading dimension N
@@ -462,9 +462,13 @@ struct Place {
 template <int BM, int BN, int HALVES>
 static __device__ inline Place place(const Args& a, int t) {
     constexpr int GM = 8, NT = BN / HALVES;
-    const bool quarter = BM == 128 && a.quarters;  // (the order of the tiles is then that of the 256 x 256 ones)
-    const int tm = quarter ? 256 : BM, tn = quarter ? 256 / HALVES : NT, corner = quarter ? t % 4 : 0;
-    t = (quarter ? t / 4 : t) + a.first;
+    int tm = BM, tn = NT, down = 1, piece = 0;
+    if (a.tm) {
+        tm = a.tm, tn = a.tn, down = tm / BM;
+        const int pieces = down * (tn / NT);
+        piece = t % pieces;
+        t = t / pieces + a.first;
+    }
     int z = 0, nm = (a.p[0].M + tm - 1) / tm, nn = (a.p[0].N + tn - 1) / tn;
     while (z + 1 < a.nprod && t >= nm * nn) {
         t -= nm * nn;
@@ -472,7 +476,7 @@ static __device__ inline Place place(const Args& a, int t) {
         nm = (a.p[z].M + tm - 1) / tm, nn = (a.p[z].N + tn - 1) / tn;
     }
     const int group = t / (GM * nn), gm0 = group * GM, gsize = nm - gm0 < GM ? nm - gm0 : GM;
-    return {z, (gm0 + (t - group * GM * nn) % gsize) * tm + corner % 2 * BM, (t - group * GM * nn) / gsize * tn + corner / 2 * NT};
+    return {z, (gm0 + (t - group * GM * nn) % gsize) * tm + (a.tm ? piece % down * BM : 0), (t - group * GM * nn) / gsize * tn + (a.tm ? piece / down * NT : 0)};
 }
 
 // STAGES: so many buffers of both operands, each step loaded that many steps ahead; 0: three of A and two of B, which is what 256 x 256 and two

@@ -67,7 +67,7 @@ constexpr Tile TILE[TILES] = {
     {32, 128, 128, 3, 3, {0.46, 0.50, 0.65}, {0.46, 0.50, 0.65}, {0.55, 1.1, 1.65}, {0.55, 1.1, 1.65}, {5, 6, 7}}};
 struct Plan {
     int which, split;  // tile; parts of K
-    int quarters;      // T256: whole rounds of them, the rest as quarters, cut into so many parts of K (0: no such rest)
+    int rest;          // not 0: a second launch does the tiles that do not fill a round, as pieces with so many parts of K
     int64_t big, all;  // tiles of the first launch; of all
 };
 int64_t tiles_of(const Args& a, int epi, int which) {
@@ -85,6 +85,10 @@ double tiles_cost(int which, int epi, int es, int64_t n, double steps) {
     return whole * (steps * c[slots - 1] + t.end[epi]) + (rest ? steps * c[rest - 1] + t.end[epi] : 0);
 }
 int64_t part_size(int which, int epi) { return (int64_t)TILE[which].bm * (epi == EPI_GATE ? TILE[which].bn_gate : TILE[which].bn) * 4; }
+// what the rest of a product is done with, and how many of them make a tile
+int piece_of(int which) { return which == T128 ? T64 : T128; }
+int cols_of(int which, int epi) { return epi == EPI_GATE ? TILE[which].bn_gate / 2 : TILE[which].bn; }
+int pieces_of(int which, int epi) { return TILE[which].bm / TILE[piece_of(which)].bm * (cols_of(which, epi) / cols_of(piece_of(which), epi)); }
 // the least that n tiles cost with K whole or cut into parts; room: bytes of workspace for them
 double cut(int which, int epi, int es, int64_t n, int total, int64_t room, int* parts) {
     double least = tiles_cost(which, epi, es, n, total);
@@ -112,11 +116,10 @@ Plan plan(const Args& a, int epi, bool ak, int es, int64_t room) {
         const int64_t n = tiles_of(a, epi, which);
         const double cost = tiles_cost(which, epi, es, n, total);
         if (cost < least) least = cost, best = {which, 1, 0, n, n};
-        if (which == T256 && n > CUS && n % CUS) {
-            const int64_t rest = n % CUS;
+        if (which <= T128 && n > CUS && n % CUS) {
             int parts;
-            const double c = tiles_cost(T256, epi, es, n - rest, total) + cut(T128, epi, es, 4 * rest, total, room, &parts) + 2;
-            if (c < least) least = c, best = {T256, 1, parts, n - rest, n};
+            const double c = tiles_cost(which, epi, es, n - n % CUS, total) + cut(piece_of(which), epi, es, pieces_of(which, epi) * (n % CUS), total, room, &parts) + 2;
+            if (c < least) least = c, best = {which, 1, parts, n - n % CUS, n};
         }
         if (which < T128) continue;
         int parts;
@@ -139,31 +142,33 @@ int launch3(ude_ctx* c, Args a, bool tile) {
     const Plan p = plan(a, EPI, AK, sizeof(typename T::E), a.room);
     if (tile && p.big * p.split < 1 << 22 && p.all < 1 << 22) {
         constexpr bool GATE = EPI == EPI_GATE, HALF = sizeof(typename T::E) == 2;
-        a.split = p.split, a.tiles = (int)p.big;
-        const dim3 grid((unsigned)(p.big * p.split)), block(256);
+        const dim3 block(256);
         auto go = [&](auto kernel, dim3 g) { hipLaunchKernelGGL(kernel, g, block, 0, c->stream, a); };
-        if constexpr (HALF) {
-            if (p.which == T256) go(gemm_tile<T, EPI, AK, BKc, 256, 256, 2, 2, 1, 0>, grid);
-            if (p.which == T256x128) go(gemm_tile<T, EPI, AK, BKc, 256, 128, 2, 2, 1, 0>, grid);
-        }
-        if (p.which == T128) go(gemm_tile<T, EPI, AK, BKc, 128, 128, 2, 2, 2, 0>, grid);
-        if (p.which == T64) go(gemm_tile<T, EPI, AK, BKc, 64, GATE ? 128 : 64, 2, 2, HALF || GATE ? 2 : 3, HALF ? (GATE ? 3 : 4) : 0>, grid);
-        if constexpr (AK)
-            if (p.which == T32) go(gemm_tile<T, EPI, AK, BKc, 32, 128, 1, 4, 3, 0>, grid);
-        HIPCHK(c, hipGetLastError());
-        if (p.quarters) {
-            const unsigned rest = (unsigned)(4 * (p.all - p.big));
-            a.first = (int)p.big, a.quarters = 1, a.split = p.quarters, a.tiles = (int)rest;
-            go(gemm_tile<T, EPI, AK, BKc, 128, 128, 2, 2, 2, 0>, dim3(rest * p.quarters));
+        // `tiles` of a kind, each cut into `split` parts
+        auto run = [&](int which, int64_t tiles, int split) {
+            a.split = split, a.tiles = (int)tiles;
+            const dim3 grid((unsigned)(tiles * split));
+            if constexpr (HALF) {
+                if (which == T256) go(gemm_tile<T, EPI, AK, BKc, 256, 256, 2, 2, 1, 0>, grid);
+                if (which == T256x128) go(gemm_tile<T, EPI, AK, BKc, 256, 128, 2, 2, 1, 0>, grid);
+            }
+            if (which == T128) go(gemm_tile<T, EPI, AK, BKc, 128, 128, 2, 2, 2, 0>, grid);
+            if (which == T64) go(gemm_tile<T, EPI, AK, BKc, 64, GATE ? 128 : 64, 2, 2, HALF || GATE ? 2 : 3, HALF ? (GATE ? 3 : 4) : 0>, grid);
+            if constexpr (AK)
+                if (which == T32) go(gemm_tile<T, EPI, AK, BKc, 32, 128, 1, 4, 3, 0>, grid);
             HIPCHK(c, hipGetLastError());
-            if (p.quarters > 1) go(join_parts<T, EPI, 128, 128, 2, 2>, dim3(rest, 4));
-            HIPCHK(c, hipGetLastError());
-        }
-        if (p.split > 1) {
-            if (p.which == T128) go(join_parts<T, EPI, 128, 128, 2, 2>, dim3((unsigned)p.big, 4));
-            if (p.which == T64) go(join_parts<T, EPI, 64, GATE ? 128 : 64, 2, 2>, dim3((unsigned)p.big, 2));
-            if (p.which == T32) go(join_parts<T, EPI, 32, 128, 1, 4>, dim3((unsigned)p.big, 2));
-            HIPCHK(c, hipGetLastError());
+            if (split > 1) {
+                if (which == T128) go(join_parts<T, EPI, 128, 128, 2, 2>, dim3((unsigned)tiles, 4));
+                if (which == T64) go(join_parts<T, EPI, 64, GATE ? 128 : 64, 2, 2>, dim3((unsigned)tiles, 2));
+                if (which == T32) go(join_parts<T, EPI, 32, 128, 1, 4>, dim3((unsigned)tiles, 2));
+                HIPCHK(c, hipGetLastError());
+            }
+            return (int)UDE_OK;
+        };
+        if (int rc = run(p.which, p.big, p.split)) return rc;
+        if (p.rest) {
+            a.first = (int)p.big, a.tm = TILE[p.which].bm, a.tn = cols_of(p.which, EPI);
+            return run(piece_of(p.which), pieces_of(p.which, EPI) * (p.all - p.big), p.rest);
         }
         return UDE_OK;
     }
