@@ -112,6 +112,22 @@ def test_products_cut_along_k(size, kind):
         assert all(torch.equal(got[k], again[k]) for k in again)
 
 
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+def test_few_rows(T, kind):
+    """at most a handful of samples: aligned rows whose last k do not fill 16 bytes, output columns that no wavefront's share divides, NaN in the
+    gaps; more k than the lanes take at once; the same bits for a sample alone and next to others of its number of rows"""
+    import universal_differential_equations_amd as U
+    for size, gap in (((T, 1021, 525, 131), 3), ((T, 3, 11, 5), 5), ((T, 2304, 1029, 64), 3), ((T, 4096, 520, 257), 0)):
+        s = made(*size, kind, True, seed=17, gap=gap)
+        check(*s)
+        x, *w = s[:4]
+        y = U.gated_ffn(x, *w)
+        assert torch.equal(y, U.gated_ffn(x, *w, save=True)[0])
+        x[1:] = 1  # (in place: a copy would have no gaps, and what is aligned is summed in another order)
+        assert torch.equal(U.gated_ffn(x, *w)[0], y[0])
+
+
 def test_against_differences():
     """directional derivatives of sum(y * c) by central differences of the Float64 statement"""
     import universal_differential_equations_amd as U

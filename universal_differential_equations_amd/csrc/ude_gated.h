@@ -645,8 +645,9 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
         f4* to = (f4*)a.part + (((int64_t)(t % tiles) * a.split + part) * NW + wave) * FM * FN * 64 + lane;
 #pragma unroll
         for (int i = 0; i < FM; ++i)
+            if (m0 + wm * (BM / NWM) + i * 16 + (lane & 15) < q.M)
 #pragma unroll
-            for (int j = 0; j < FN; ++j) to[(i * FN + j) * 64] = acc[i][j];
+                for (int j = 0; j < FN; ++j) to[(i * FN + j) * 64] = acc[i][j];
         return;
     }
     // epilogue: 32 rows of a wavefront at a time through LDS, so that the code of finish() stands in a loop and a row's lanes store side by
@@ -691,6 +692,7 @@ __global__ __launch_bounds__(64 * NWM * NWN) void join_parts(const Args a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % NWM, wn = wave / NWM, i = blockIdx.y;
     const Place at = place<BM, BN, HALVES>(a, (int)blockIdx.x);
     const Product& q = a.p[at.z];
+    if (at.m0 + wm * (BM / NWM) + i * 16 + (lane & 15) >= q.M) return;  // (rows outside have no parts)
     const f4* from = (const f4*)a.part + (((int64_t)blockIdx.x * a.split) * NW + wave) * FM * FN * 64 + i * FN * 64 + lane;
     f4 sum[FN] = {};
 #pragma unroll 8
@@ -708,6 +710,80 @@ __global__ __launch_bounds__(64 * NWM * NWN) void join_parts(const Args a) {
         v[j] = sum[j + FN - N];
     }
     finish<T, EPI, N>(a, q, m, n, c, v);
+}
+
+// ---- a few rows ------------------------------------------------------------------------------------------------------------------------
+// C[m, n] = sum_k A(m, k) B(n, k) for at most ROWS rows of A where B's k are adjacent: a wavefront for NB rows of B (EPI_GATE: half of them of Wg, half
+// of Wu), 16 bytes of k a lane, sums in Float32 over the lanes at the end.  Bound by reading B, once and in full lines: a tile of matrix instructions
+// does that too, but has to cut K to fill the card and join the parts in launches of their own.  One row through a block of 4096 x 11264 in
+// BFloat16 takes 44.5 us = 6.2 TB/s (32 x 128 tiles: 67), four rows 68 (68), in Float32 116 (139); through 2048 x 5632 18 us (31) and 26 (31).  With more
+// rows the loads of A and the conversions outweigh those of B (eight rows: 150 us): four rows of B a wavefront instead of two took two
+// rows from 64 to 57 us and four from 89 to 68.
+template <int EPI, int ROWS>
+struct Few {
+    static constexpr int NB = ROWS == 1 ? 2 : 4, HALVES = EPI == EPI_GATE ? 2 : 1, NT = NB / HALVES;  // rows of B; output columns
+};
+template <class T, int EPI, int ROWS>
+__global__ __launch_bounds__(256) void few_rows(const Args a) {
+    typedef typename T::E E;
+    constexpr int V = 16 / (int)sizeof(E), NB = Few<EPI, ROWS>::NB, HALVES = Few<EPI, ROWS>::HALVES, NT = Few<EPI, ROWS>::NT;
+    typedef E EV __attribute__((ext_vector_type(V)));
+    touch(a);
+    const Product& q = a.p[0];
+    const int lane = threadIdx.x & 63, n0 = ((int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * NT;
+    if (n0 >= q.N) return;
+    const E *b[NB], *x[ROWS];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {  // (columns outside: the first one again, not stored)
+        const Product& p = a.p[j / NT];
+        b[j] = (const E*)p.B + (int64_t)(n0 + j % NT < q.N ? n0 + j % NT : n0) * p.ldb;
+    }
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m) x[m] = (const E*)q.A + (m < q.M ? m : 0) * q.lda;
+    float s[ROWS][NB] = {};
+#pragma unroll (ROWS == 1 ? 4 : 2)
+    for (int k = lane * V; k <= a.K - V; k += 64 * V) {
+        EV w[NB], y[ROWS];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) w[j] = __builtin_nontemporal_load((const EV*)(b[j] + k));
+#pragma unroll
+        for (int m = 0; m < ROWS; ++m) y[m] = *(const EV*)(x[m] + k);
+#pragma unroll
+        for (int m = 0; m < ROWS; ++m)
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+#pragma unroll
+                for (int j = 0; j < NB; ++j) s[m][j] = fmaf(T::to(y[m][e]), T::to(w[j][e]), s[m][j]);
+    }
+    if (const int k = a.K / V * V + lane; k < a.K) {
+#pragma unroll
+        for (int m = 0; m < ROWS; ++m)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) s[m][j] = fmaf(T::to(x[m][k]), T::to(b[j][k]), s[m][j]);
+    }
+    float c[NB];
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+#pragma unroll
+            for (int d = 32; d; d >>= 1) s[m][j] += __shfl_xor(s[m][j], d);
+            c[j] = lane == m ? s[m][j] : m ? c[j] : 0.f;
+        }
+    if (lane >= q.M) return;  // lane m stores row m
+    E* to = (E*)q.C + lane * q.ldc + n0;
+    float act[NT], slope[NT];
+    if constexpr (EPI == EPI_GATE) gate_acts<sizeof(E) == 2, NT>(a.act, c, act, slope);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        if (n0 + j >= q.N) return;
+        if constexpr (EPI == EPI_GATE) {
+            to[j] = T::from(act[j] * c[j + NT]);
+            if (a.gate) a.gate[(int64_t)lane * q.N + n0 + j] = c[j], a.up[(int64_t)lane * q.N + n0 + j] = c[j + NT];
+        } else {
+            to[j] = T::from(c[j]);
+        }
+    }
 }
 
 }  // namespace gated

@@ -128,6 +128,7 @@ Plan plan(const Args& a, int epi, bool ak, int es, int64_t room) {
     }
     return best;
 }
+constexpr int MOST_FEW = 4;  // rows of A that few_rows is faster for than tiles, or as fast (both sides: there)
 // no product of these sizes, nor some of `n` such products side by side, leaves more bytes of parts than this
 int64_t part_bytes(int64_t M, int64_t N, int64_t steps, int n) {
     const int64_t all = n * ((M + 127) / 128) * ((N + 63) / 64) * (steps / 2);  // (part bytes of a tile go with its area: the largest tile's)
@@ -139,6 +140,17 @@ bool tileable(const void* p, int64_t ld, int e) { return (uintptr_t)p % 4 == 0 &
 
 template <class T, int EPI, bool AK, bool BKc>
 int launch3(ude_ctx* c, Args a, bool tile) {
+    if constexpr (EPI != EPI_PULL && AK && BKc) {
+        const int M = a.p[0].M;
+        if (M <= MOST_FEW && a.nprod == 1 && a.nseg == 1 && a.p[0].vecA && a.p[0].vecB && (EPI != EPI_GATE || a.p[1].vecB)) {
+            auto go = [&](auto kernel, int columns) { hipLaunchKernelGGL(kernel, dim3((unsigned)((a.p[0].N + 4 * columns - 1) / (4 * columns))), dim3(256), 0, c->stream, a); };
+            if (M == 1) go(few_rows<T, EPI, 1>, Few<EPI, 1>::NT);
+            else if (M == 2) go(few_rows<T, EPI, 2>, Few<EPI, 2>::NT);
+            else go(few_rows<T, EPI, 4>, Few<EPI, 4>::NT);
+            HIPCHK(c, hipGetLastError());
+            return UDE_OK;
+        }
+    }
     const Plan p = plan(a, EPI, AK, sizeof(typename T::E), a.room);
     if (tile && p.big * p.split < 1 << 22 && p.all < 1 << 22) {
         constexpr bool GATE = EPI == EPI_GATE, HALF = sizeof(typename T::E) == 2;
