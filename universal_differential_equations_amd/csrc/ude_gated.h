@@ -683,33 +683,37 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
     }
 }
 
-// Adds up the parts of K of a tile, in their order, and does what the tile kernel would have done with the sums.  One wavefront per 16 rows of
-// a wavefront's tile; the parts lie as the lanes held them, so that every access is one contiguous 1 KB.
+// Adds up the parts of K of a tile, in their order, and does what the tile kernel would have done with the sums.  One wavefront per 16 x 16 of
+// a wavefront's tile (EPI_GATE: two of them, of gate and of up); the parts lie as the lanes held them, so that every access is one contiguous
+// 1 KB.  Bound by the way to memory and back: 8 parts at once.
 template <class T, int EPI, int BM, int BN, int NWM, int NWN>
 __global__ __launch_bounds__(64 * NWM * NWN) void join_parts(const Args a) {
     constexpr int NW = NWM * NWN, FM = BM / NWM / 16, FN = BN / NWN / 16, HALVES = EPI == EPI_GATE ? 2 : 1, NT = BN / HALVES;
     touch(a);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % NWM, wn = wave / NWM, i = blockIdx.y;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave % NWM, wn = wave / NWM, i = blockIdx.y, j = blockIdx.z;
     const Place at = place<BM, BN, HALVES>(a, (int)blockIdx.x);
     const Product& q = a.p[at.z];
-    if (at.m0 + wm * (BM / NWM) + i * 16 + (lane & 15) >= q.M) return;  // (rows outside have no parts)
-    const f4* from = (const f4*)a.part + (((int64_t)blockIdx.x * a.split) * NW + wave) * FM * FN * 64 + i * FN * 64 + lane;
-    f4 sum[FN] = {};
-#pragma unroll 8
-    for (int s = 0; s < a.split; ++s)
+    const int m[1] = {at.m0 + wm * (BM / NWM) + i * 16 + (lane & 15)}, n[1] = {at.n0 + wn * (NT / NWN) + j * 16 + (lane >> 4) * 4};
+    if (m[0] >= q.M) return;  // (rows outside have no parts)
+    const f4* from = (const f4*)a.part + (((int64_t)blockIdx.x * a.split) * NW + wave) * FM * FN * 64 + (i * FN + j) * 64 + lane;
+    f4 c[1] = {}, v[1] = {};
+    constexpr int U = 8;
+    for (int s = 0; s < a.split; s += U) {
+        f4 x[U], y[U];
 #pragma unroll
-        for (int j = 0; j < FN; ++j) sum[j] += from[((int64_t)s * NW * FM * FN + j) * 64];
-    constexpr int N = FN / HALVES;
-    int m[N], n[N];
-    f4 c[N], v[N];
+        for (int u = 0; u < U; ++u) {  // (behind the last one: that again, not added)
+            const f4* p = from + (int64_t)(s + u < a.split ? s + u : a.split - 1) * (NW * FM * FN * 64);
+            x[u] = p[0];
+            if constexpr (HALVES == 2) y[u] = p[FN / 2 * 64];
+        }
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        m[j] = at.m0 + wm * (BM / NWM) + i * 16 + (lane & 15);
-        n[j] = at.n0 + wn * (NT / NWN) + j * 16 + (lane >> 4) * 4;
-        c[j] = sum[j];
-        v[j] = sum[j + FN - N];
+        for (int u = 0; u < U; ++u)
+            if (s + u < a.split) {
+                c[0] += x[u];
+                if constexpr (HALVES == 2) v[0] += y[u];
+            }
     }
-    finish<T, EPI, N>(a, q, m, n, c, v);
+    finish<T, EPI, 1>(a, q, m, n, c, v);
 }
 
 // ---- a few rows ------------------------------------------------------------------------------------------------------------------------

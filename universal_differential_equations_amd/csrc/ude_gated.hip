@@ -47,7 +47,8 @@ int vec(const void* p, int64_t ld, int e) { return (uintptr_t)p % 16 == 0 && ld 
 //   The smaller ones leave less of the last round idle, but a step costs them 0.25 to 0.5 however little there is in it (LDS, barrier, the
 //   loads' way: 64 x 64 takes 0.25 with its loads four steps ahead, 0.41 with two), so that they are for small products, and for Float32, whose matrix instructions (1/16 of the 16-bit rate) bound it with
 //   any tile.
-// EPI_GATE writes ten bytes an element at the end, EPI_PULL reads eight and writes six.  Where tiles are few and K is long, K is cut into
+// EPI_GATE writes ten bytes an element at the end, EPI_PULL reads eight and writes six: with one workgroup on a compute unit nothing is
+// multiplied meanwhile, so that a pull of 4096 x 5632 x 2048 is done in 159 us by 128 x 128 tiles, 171 by 256 x 256 and pieces, 185 by 256 x 128.  Where tiles are few and K is long, K is cut into
 // parts whose sums go through memory (3 TB/s) and one more launch.
 constexpr int CUS = 256;
 constexpr int64_t MOST_PART_BYTES = (int64_t)2 * CUS * 128 * 128 * 4;
@@ -60,9 +61,9 @@ struct Tile {
     double end[3];                   // EPI_STORE, EPI_GATE, EPI_PULL
 };
 constexpr Tile TILE[TILES] = {
-    {256, 256, 256, 1, 1, {1.46}, {1.46}, {}, {}, {12, 20, 45}},
-    {256, 128, 128, 1, 1, {0.85}, {0.85}, {}, {}, {9, 13, 28}},
-    {128, 128, 128, 2, 2, {0.48, 1.02}, {0.48, 1.02}, {1.95, 3.8}, {1.95, 3.8}, {7, 9, 17}},
+    {256, 256, 256, 1, 1, {1.46}, {1.46}, {}, {}, {12, 20, 60}},
+    {256, 128, 128, 1, 1, {0.85}, {0.85}, {}, {}, {9, 13, 34}},
+    {128, 128, 128, 2, 2, {0.48, 1.02}, {0.48, 1.02}, {1.95, 3.8}, {1.95, 3.8}, {7, 9, 20}},
     {64, 64, 128, 2, 3, {0.25, 0.43}, {0.40, 0.64}, {0.54, 1.08, 1.6}, {1.08, 2.1, 3.2}, {5, 6, 7}},
     {32, 128, 128, 3, 3, {0.46, 0.50, 0.65}, {0.46, 0.50, 0.65}, {0.55, 1.1, 1.65}, {0.55, 1.1, 1.65}, {5, 6, 7}}};
 struct Plan {
@@ -170,9 +171,9 @@ int launch3(ude_ctx* c, Args a, bool tile) {
                 if (which == T32) go(gemm_tile<T, EPI, AK, BKc, 32, 128, 1, 4, 3, 0>, grid);
             HIPCHK(c, hipGetLastError());
             if (split > 1) {
-                if (which == T128) go(join_parts<T, EPI, 128, 128, 2, 2>, dim3((unsigned)tiles, 4));
-                if (which == T64) go(join_parts<T, EPI, 64, GATE ? 128 : 64, 2, 2>, dim3((unsigned)tiles, 2));
-                if (which == T32) go(join_parts<T, EPI, 32, 128, 1, 4>, dim3((unsigned)tiles, 2));
+                if (which == T128) go(join_parts<T, EPI, 128, 128, 2, 2>, dim3((unsigned)tiles, 4, GATE ? 2 : 4));
+                if (which == T64) go(join_parts<T, EPI, 64, GATE ? 128 : 64, 2, 2>, dim3((unsigned)tiles, 2, 2));
+                if (which == T32) go(join_parts<T, EPI, 32, 128, 1, 4>, dim3((unsigned)tiles, 2, GATE ? 1 : 2));
                 HIPCHK(c, hipGetLastError());
             }
             return (int)UDE_OK;
