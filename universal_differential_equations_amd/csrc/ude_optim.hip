@@ -215,21 +215,28 @@ __global__ __launch_bounds__(256) void adamw32_kernel(const AdamArgs a) {
 // (the same squared).  A Float32 root, less what it may be too large by, gives q or q - 1; the border between the two is a whole number
 // plus 1/4 below 2^17 (exact in Float32; its square has at most 38 bits) and is compared with y in Float64.
 __device__ inline int code_m(double y) {
-    const int q = (int)(__builtin_amdgcn_sqrtf((float)y) + 0.4999f);  // roots up to 127, a few 2^-24 of them off
-    const float border = (float)(q * q + q) + 0.25f;
-    const int r = y >= (double)border ? q + 1 : q;
+    const float q = truncf(__builtin_amdgcn_sqrtf((float)y) + 0.4999f);  // roots up to 127, a few 2^-24 of them off
+    const int r = (int)q + (y >= (double)(fmaf(q, q, q) + 0.25f));
     return r > 127 ? 127 : r;
 }
 __device__ inline int code_v(double y) {
-    const int q = (int)(__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)y)) + 0.499f);
-    const double border = (double)((float)(q * q + q) + 0.25f);
-    const int r = y >= border * border ? q + 1 : q;
+    const float q = truncf(__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)y)) + 0.499f);
+    const double border = (double)(fmaf(q, q, q) + 0.25f);
+    const int r = (int)q + (y >= border * border);
     return r > 255 ? 255 : r == 0 && y > 0 ? 1 : r;
 }
 // what a code stands for, over the scale: signed squares of up to 14 bits, fourth powers of up to 32
 __device__ inline double m_part(int q) { return (double)(q * (q < 0 ? -q : q)); }
 __device__ inline double v_part(int r) { return (double)((unsigned)(r * r) * (unsigned)(r * r)); }
 constexpr double M_UNIT = 1.0 / 16129.0, V_UNIT = 1.0 / 4228250625.0;
+
+// root of x >= 0 and 1 / x by the hardware's instructions, 2^-23 of the value off (measured over every float: 1.56 and 1.54 2^-24); what they take
+// for zero is scaled first.  A step has a dozen roundings of 2^-24 besides.
+__device__ inline float quick_root(float x) {
+    const bool tiny = x < 0x1p-96f;
+    const float r = __builtin_amdgcn_sqrtf(tiny ? x * 0x1p64f : x);
+    return tiny ? r * 0x1p-32f : r;
+}
 
 // the largest of 16 lanes' values, as whole numbers (that is the order of floats >= 0, and above them infinity and NaN), by rotations in a row of 16
 __device__ inline int row_max(int x) {
@@ -317,7 +324,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(const AdamArgs a) {
         mm[i] = (int8_t)(m[i] < 0 ? -q : q);
         vv[i] = (uint8_t)code_v(v[i] * ic);
         float w = master ? ww[i] : (float)pp[i];
-        w = w * keep - rate * (float)m[i] / (sqrtf((float)v[i] * rc2) + eps);
+        w = w * keep - rate * (float)m[i] * __builtin_amdgcn_rcpf(quick_root((float)v[i] * rc2) + eps);
         ww[i] = w;
         pp[i] = (PE)w;
     }
