@@ -424,16 +424,13 @@ __device__ inline double block_sum(double x) {
     return all;
 }
 
-// thread t of 256 adds its 16 elements of chunk c: 16-byte loads side by side where the tensor allows it, all of them before the first use
-template <class G>
-__device__ inline void add_chunk(const NormArgs& a, int c, int t, double* sum) {
-    typedef typename G::E E;
+// the 16 elements of chunk c, of tensor k, that thread t of 256 adds: 16-byte loads side by side where the tensor allows it
+template <class E>
+__device__ inline void get_chunk(const NormArgs& a, int k, int c, int t, E* x) {
     constexpr int V = 16 / sizeof(E);
-    const int k = tensor_of(a, c);
     const int64_t at = (int64_t)(c - a.first[k]) * NORM_CHUNK;
     const int64_t end = a.n[k] < at + NORM_CHUNK ? a.n[k] : at + NORM_CHUNK;
     const E* g = (const E*)a.g[k];
-    E x[16];
     if (end == at + NORM_CHUNK && fits<V>(g)) {
 #pragma unroll
         for (int j = 0; j < 16 / V; ++j) get<V>(g + at + j * 256 * V + t * V, x + j * V);
@@ -444,6 +441,9 @@ __device__ inline void add_chunk(const NormArgs& a, int c, int t, double* sum) {
             x[j] = i < end ? g[i] : (E)0;
         }
     }
+}
+template <class G>
+__device__ inline void add_squares(const typename G::E* x, double* sum) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
         const double y = (double)(typename G::W)x[j];
@@ -456,12 +456,16 @@ __device__ inline void write_norm(double sum, double max_norm, double* out) {
     out[1] = !(max_norm > 0) ? (norm != norm ? norm : 1) : norm <= max_norm ? 1 : max_norm / norm;
 }
 
-// Bound by reading: 277 MB of BFloat16 in 42 us = 6.6 TB/s, the sum of the workgroups' sums 4 us more.  Squares and sums in Float64: nothing
-// overflows before the norm does, and the order of the sums does not show.
+// Bound by reading: 277 MB of BFloat16 in 42 us = 6.6 TB/s, the sum of the workgroups' sums 4 us more.  Squares and sums in Float64, where those
+// of smaller types neither overflow nor vanish.
 template <class G>
 __global__ __launch_bounds__(256) void norm_part_kernel(const NormArgs a) {
     double sum[4] = {};
-    for (int c = (int)blockIdx.x; c < a.chunks; c += (int)gridDim.x) add_chunk<G>(a, c, threadIdx.x, sum);
+    for (int c = (int)blockIdx.x; c < a.chunks; c += (int)gridDim.x) {
+        typename G::E x[16];
+        get_chunk(a, tensor_of(a, c), c, threadIdx.x, x);
+        add_squares<G>(x, sum);
+    }
     const double all = block_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
     if (threadIdx.x == 0) a.part[blockIdx.x] = all;
 }
@@ -473,11 +477,33 @@ __global__ __launch_bounds__(256) void norm_join_kernel(const double* part, int 
     if (threadIdx.x == 0) write_norm(sum, max_norm, out);
 }
 
-// few chunks: one workgroup, four chunks at a time, and no second launch (which costs more than what one compute unit takes for them)
+// few chunks: one workgroup, four chunks side by side, four (Float64: two) such rounds in flight, and no second launch (which costs more than what one compute unit takes for them).  The tensor of
+// a chunk is counted out of all that begin before it: looked up in the arguments step by step, it took longer than the sums.
 template <class G>
 __global__ __launch_bounds__(1024) void norm_one_kernel(const NormArgs a, double max_norm, double* out) {
+    constexpr int L = (NORM_NT + 63) / 64;
+    int first[L];  // lane l: where the tensors l, l + 64, .. begin
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+        const int k = i * 64 + (threadIdx.x & 63);
+        first[i] = k < a.nt ? a.first[k] : INT32_MAX;
+    }
     double sum[4] = {};
-    for (int c = threadIdx.x >> 8; c < a.chunks; c += 4) add_chunk<G>(a, c, threadIdx.x & 255, sum);
+    constexpr int U = sizeof(typename G::E) == 8 ? 2 : 4;
+    for (int c0 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8); c0 < a.chunks; c0 += 4 * U) {
+        typename G::E x[U][16];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int c = c0 + 4 * u;
+            int k = -1;
+#pragma unroll
+            for (int i = 0; i < L; ++i) k += __popcll(__ballot(first[i] <= c));
+            if (c < a.chunks) get_chunk(a, k, c, threadIdx.x & 255, x[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (c0 + 4 * u < a.chunks) add_squares<G>(x[u], sum);
+    }
     const double all = block_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
     if (threadIdx.x == 0) write_norm(all, max_norm, out);
 }
