@@ -128,6 +128,15 @@ def test_few_rows(T, kind):
         assert torch.equal(U.gated_ffn(x, *w)[0], y[0])
 
 
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+def test_broadcast_samples_and_cotangents(kind):
+    """x and dy as views whose rows are one row, one column among them: what sums and means hand back"""
+    for size in ((40, 24, 30, 1), (40, 1, 30, 7)):
+        x, wg, wu, wd, dy = made(*size, kind, True, seed=18)
+        check(x[:1].expand(40, -1), wg, wu, wd, dy[:1].expand(40, -1))
+        check(x, wg, wu, wd, dy[:1, :1].expand(40, size[3]))
+
+
 def test_against_differences():
     """directional derivatives of sum(y * c) by central differences of the Float64 statement"""
     import universal_differential_equations_amd as U

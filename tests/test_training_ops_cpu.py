@@ -120,3 +120,20 @@ def test_flux_adamw_tag():
     assert (o.eta, o.beta, o.decay, o.max_norm, o.eps) == (0.03, (0.9, 0.999), 0.01, 1.0, 1e-8)
     with pytest.raises(ValueError):
         pde.ADAMW(0.0)
+
+
+@pytest.mark.parametrize("make", [lambda t: t.ones(1, 1).expand(5, 1), lambda t: t.ones(1, 3).expand(5, 3), lambda t: t.ones(5, 1).expand(5, 3),
+                                  lambda t: t.arange(9.).as_strided((5, 3), (1, 1)), lambda t: t.arange(15.).view(3, 5).T, lambda t: t.ones(9, 3)[::2],
+                                  lambda t: t.ones(5, 4)[:, :1], lambda t: t.ones(7, 3)[2:3], lambda t: t.ones(1, 3).as_strided((1, 3), (2 ** 40, 1))],
+                         ids=["broadcast column", "broadcast row", "broadcast columns", "overlapping", "transposed", "every other row", "a column", "a row",
+                              "a row with a far next"])
+def test_rows_of_any_view(make):
+    """what the kernels read through (address, leading dimension) is the tensor, for every view that x or dy may be"""
+    from universal_differential_equations_amd import layers
+    x = make(torch)
+    y = layers._rows(x)
+    n, cols = y.shape
+    ld = layers._row_ld(y)
+    last = (n - 1) * ld + cols  # the last element that is read, in the storage
+    assert ld >= cols and y.storage_offset() + last <= y.untyped_storage().nbytes() // y.element_size()
+    assert torch.equal(y.as_strided((n, cols), (ld, 1)), x)

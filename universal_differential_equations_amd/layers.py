@@ -76,7 +76,7 @@ class _Block:
         self.torch, self.shape, self.device, self.dtype = torch, x.shape, dev, dtype
         self.x = _rows(x if x.dim() == 2 else x.reshape(-1, d))
         self.w = (w_gate, w_up, w_down)
-        self.D = _lib.GatedFfnDesc(code, gate, order, 0, self.x.shape[0], d, f, o, max(self.x.stride(0), d), o,
+        self.D = _lib.GatedFfnDesc(code, gate, order, 0, self.x.shape[0], d, f, o, _row_ld(self.x), o,
                                    _ld(w_gate, order), _ld(w_up, order), _ld(w_down, order))
         self.eng = Engine.get(dev.index)
 
@@ -93,8 +93,14 @@ class _Block:
 
 
 def _rows(x):
-    """x with contiguous rows (copied where it has not)"""
-    return x if x.shape[1] == 1 or (x.stride(1) == 1 and (x.stride(0) >= x.shape[1] or x.shape[0] <= 1)) else x.contiguous()
+    """x with contiguous rows that do not overlap (copied where it has not)"""
+    (rows, cols), (r, c) = x.shape, x.stride()
+    return x if (c == 1 or cols == 1) and (r >= cols or rows <= 1) else x.contiguous()
+
+
+def _row_ld(x):
+    """elements from one row of `_rows`' result to the next (of a single row: without gaps, whatever its stride says)"""
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
 def _p(t):
@@ -134,7 +140,7 @@ def gated_ffn_pullback(saved, dy, need=("x", "w_gate", "w_up", "w_down")):
         raise ValueError("gated_ffn_pullback: need has %s" % sorted(unknown))
     dy = _rows(dy if dy.dim() == 2 else dy.reshape(-1, b.D.O))
     D = _lib.GatedFfnDesc.from_buffer_copy(b.D)
-    D.ldy = max(dy.stride(0), D.O)
+    D.ldy = _row_ld(dy)
     t, f = D.T, D.F
     dx = torch.empty((t, D.D), dtype=b.dtype, device=b.device) if "x" in need else None
     grads = []
