@@ -137,6 +137,25 @@ def test_broadcast_samples_and_cotangents(kind):
         check(x, wg, wu, wd, dy[:1, :1].expand(40, size[3]))
 
 
+def test_very_many_columns():
+    """one sample through more hidden columns than a launch of one wavefront per column could have, and a product as long as that: the columns
+    at both ends and the one that the output is made of"""
+    import universal_differential_equations_amd as U
+    D, F = 8, (1 << 26) + 24
+    x, dt = torch.linspace(-1, 1, D, device="cuda").view(1, D).bfloat16(), torch.bfloat16
+    wg, wu = torch.empty((F, D), dtype=dt, device="cuda").normal_(), torch.empty((F, D), dtype=dt, device="cuda").normal_()
+    wd = torch.zeros((1, F), dtype=dt, device="cuda")
+    wd[0, F - 3] = 1
+    y, saved = U.gated_ffn(x, wg, wu, wd, act="identity", save=True)
+    for at in (0, F // 2, 1 << 25, F - 64):
+        for got, w in zip(saved.gate, (wg, wu)):
+            p = w[at:at + 64].double() * x.double()
+            # eight products, each exact in Float32, and at most eight sums
+            assert bool(((got[0, at:at + 64].double() - p.sum(1)).abs() <= 8 * 2.0 ** -24 * p.abs().sum(1)).all()), at
+    h = (saved.gate[0, 0, F - 3] * saved.gate[1, 0, F - 3]).to(dt)
+    assert torch.equal(y[0, 0], h)
+
+
 def test_against_differences():
     """directional derivatives of sum(y * c) by central differences of the Float64 statement"""
     import universal_differential_equations_amd as U
@@ -303,4 +322,39 @@ def test_two_threads():
     ts = [threading.Thread(target=go, args=(i,)) for i in (0, 1)]
     [t.start() for t in ts]
     [t.join() for t in ts]
+    assert not bad
+
+
+def test_pullback_in_another_thread_and_stream():
+    """what is saved in one thread and stream is pulled back in others, two at a time, while the first goes on: each thread has a context of its
+    own, and the saved activations' memory is not reused before the other stream has read them"""
+    import threading
+    import universal_differential_equations_amd as U
+    sets = [made(90, 72, 104, 40, torch.float32, True, seed=s) for s in (12, 13)]
+    want = [U.gated_ffn_pullback(U.gated_ffn(*s[:4], save=True)[1], s[4]) for s in sets]
+    torch.cuda.synchronize()
+    bad = []
+
+    def go(i, saved, ready):
+        stream = torch.cuda.Stream()
+        stream.wait_event(ready)
+        with torch.cuda.stream(stream):
+            got = U.gated_ffn_pullback(saved, sets[i][4])
+            del saved
+            stream.synchronize()
+            if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                bad.append(i)
+
+    for _ in range(10):
+        ts = []
+        for i in (0, 1):
+            y, saved = U.gated_ffn(*sets[i][:4], save=True)
+            ready = torch.cuda.Event()
+            ready.record()
+            ts.append(threading.Thread(target=go, args=(i, saved, ready)))
+            del y, saved
+        [t.start() for t in ts]
+        for _ in range(5):
+            torch.full((2, 90, 104), float("nan"), device="cuda")  # (the size of what was saved)
+        [t.join() for t in ts]
     assert not bad

@@ -129,7 +129,22 @@ Plan plan(const Args& a, int epi, bool ak, int es, int64_t room) {
     }
     return best;
 }
-constexpr int MOST_FEW = 4;  // rows of A that few_rows is faster for than tiles, or as fast (both sides: there)
+// Whether few_rows takes a product of up to four rows, and the tiles the others.  A wavefront has its rows of B to itself, so that few and long ones
+// take as long as their steps do one after the other, and many short ones as long as their starts and sums over the lanes: microseconds of a
+// step, and of 1024 wavefronts, as measured for one, two and four rows (128 x 2048 x 64 to 128 x 65536 x 2048).  The tiles cut K where it is
+// long, for 8 us of joining.  One row of BFloat16, K x N: 8192 x 64 in 10 us (tiles: 15), 32768 x 64 in 30 (24), 16384 x 2048 in 24 (31), 65536 x 2048
+// in 85 (72), 128 x 32768 in 14 (6); four rows: 2048 x 64 in 11 (12), 8192 x 64 in 23 (15).
+constexpr double FEW_STEP[3] = {0.5, 0.6, 1.0}, FEW_STEP32[3] = {0.25, 0.43, 0.84}, FEW_WAVES[3] = {0.44, 0.75, 1.1};
+bool few(const Args& a, int epi, int es, bool tile) {
+    const Product& p = a.p[0];
+    if (p.M > 4 || a.nprod > 1 || a.nseg > 1 || !p.vecA || !p.vecB || (epi == EPI_GATE && !a.p[1].vecB)) return false;
+    if (p.N >= 1 << 25) return false;  // (a launch has fewer than 2^32 threads, 64 for a column at most)
+    const int rows = p.M == 1 ? 0 : p.M == 2 ? 1 : 2;
+    const double steps = a.K * (es / 1024.0), waves = (double)p.N * (epi == EPI_GATE ? 2 : 1) / (rows ? 4 : 2);
+    const double one = steps * (es == 4 ? FEW_STEP32 : FEW_STEP)[rows], all = waves / 1024 * FEW_WAVES[rows];
+    const double read = (double)p.N * a.K * es * (epi == EPI_GATE ? 2 : 1) / 5.7e6, tiles = (0.2 * steps > read ? 0.2 * steps : read) + (steps < 1 ? 3 : 8);
+    return !tile || (one > all ? one : all) <= tiles;
+}
 // no product of these sizes, nor some of `n` such products side by side, leaves more bytes of parts than this
 int64_t part_bytes(int64_t M, int64_t N, int64_t steps, int n) {
     const int64_t all = n * ((M + 127) / 128) * ((N + 63) / 64) * (steps / 2);  // (part bytes of a tile go with its area: the largest tile's)
@@ -142,8 +157,8 @@ bool tileable(const void* p, int64_t ld, int e) { return (uintptr_t)p % 4 == 0 &
 template <class T, int EPI, bool AK, bool BKc>
 int launch3(ude_ctx* c, Args a, bool tile) {
     if constexpr (EPI != EPI_PULL && AK && BKc) {
-        const int M = a.p[0].M;
-        if (M <= MOST_FEW && a.nprod == 1 && a.nseg == 1 && a.p[0].vecA && a.p[0].vecB && (EPI != EPI_GATE || a.p[1].vecB)) {
+        if (few(a, EPI, sizeof(typename T::E), tile)) {
+            const int M = a.p[0].M;
             auto go = [&](auto kernel, int columns) { hipLaunchKernelGGL(kernel, dim3((unsigned)((a.p[0].N + 4 * columns - 1) / (4 * columns))), dim3(256), 0, c->stream, a); };
             if (M == 1) go(few_rows<T, EPI, 1>, Few<EPI, 1>::NT);
             else if (M == 2) go(few_rows<T, EPI, 2>, Few<EPI, 2>::NT);

@@ -78,18 +78,28 @@ class _Block:
         self.w = (w_gate, w_up, w_down)
         self.D = _lib.GatedFfnDesc(code, gate, order, 0, self.x.shape[0], d, f, o, _row_ld(self.x), o,
                                    _ld(w_gate, order), _ld(w_up, order), _ld(w_down, order))
-        self.eng = Engine.get(dev.index)
+        self.gate, self.stream = None, current_raw_stream(dev.index)
+
+    @property
+    def eng(self):
+        return Engine.get(self.device.index)
 
     def workspace(self, pullback):
         n = C.c_int64(0)
-        rc = self.eng.L.ude_gated_ffn_workspace(C.byref(self.D), pullback, C.byref(n))
+        rc = _lib.load().ude_gated_ffn_workspace(C.byref(self.D), pullback, C.byref(n))
         if rc:
             raise _lib.UdeError(rc, "gated_ffn: sizes T = %d, D = %d, F = %d, O = %d" % (self.D.T, self.D.D, self.D.F, self.D.O))
         # (from torch's allocator on the current stream: a captured call gets memory of its graph, two calls never share one)
         return self.torch.empty(max(n.value, 256), dtype=self.torch.uint8, device=self.device), n.value
 
     def bind(self):
-        self.eng.set_stream(current_raw_stream(self.device.index))
+        """this thread's context, on the current stream"""
+        eng, stream = self.eng, current_raw_stream(self.device.index)
+        eng.set_stream(stream)
+        if stream != self.stream and self.gate is not None:
+            # (saved on the forward call's stream: its memory is not given away before this one is done with it)
+            self.gate.record_stream(self.torch.cuda.current_stream(self.device))
+        return eng
 
 
 def _rows(x):
@@ -119,9 +129,9 @@ def gated_ffn(x, w_gate, w_up, w_down, act="swish", save=False):
     b.gate = torch.empty((2, t, f), dtype=torch.float32, device=b.device) if save else None
     gate = b.gate.data_ptr() if save else None
     ws, size = b.workspace(0)
-    b.bind()
-    b.eng.check(b.eng.L.ude_gated_ffn_forward_dev(b.eng.h, C.byref(D), b.x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
-                                                  y.data_ptr(), gate, gate + 4 * t * f if save else None, ws.data_ptr(), size))
+    eng = b.bind()
+    eng.check(eng.L.ude_gated_ffn_forward_dev(eng.h, C.byref(D), b.x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
+                                              y.data_ptr(), gate, gate + 4 * t * f if save else None, ws.data_ptr(), size))
     if x.dim() != 2:
         y = y.view(*b.shape[:-1], o)
     return (y, b) if save else y
@@ -150,9 +160,9 @@ def gated_ffn_pullback(saved, dy, need=("x", "w_gate", "w_up", "w_down")):
         grads.append(g if g is None or D.w_order else g.T)
     ws, size = b.workspace(1)
     gate = b.gate.data_ptr()
-    b.bind()
-    b.eng.check(b.eng.L.ude_gated_ffn_backward_dev(b.eng.h, C.byref(D), b.x.data_ptr(), *[w.data_ptr() for w in b.w], gate, gate + 4 * t * f, dy.data_ptr(),
-                                                   _p(dx), _p(grads[0]), _p(grads[1]), _p(grads[2]), ws.data_ptr(), size))
+    eng = b.bind()
+    eng.check(eng.L.ude_gated_ffn_backward_dev(eng.h, C.byref(D), b.x.data_ptr(), *[w.data_ptr() for w in b.w], gate, gate + 4 * t * f, dy.data_ptr(),
+                                               _p(dx), _p(grads[0]), _p(grads[1]), _p(grads[2]), ws.data_ptr(), size))
     if dx is not None and dx.shape != b.shape:
         dx = dx.view(b.shape)
     return (dx, *grads)
