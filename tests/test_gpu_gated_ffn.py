@@ -137,6 +137,15 @@ def test_broadcast_samples_and_cotangents(kind):
         check(x, wg, wu, wd, dy[:1, :1].expand(40, size[3]))
 
 
+@pytest.mark.parametrize("rows", [True, False], ids=["rows", "cols"])
+@pytest.mark.parametrize("size", [(6, 29, 45, 13), (70, 61, 45, 93), (300, 1021, 525, 1029), (2061, 1021, 525, 2061), (1101, 93, 4101, 61)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+def test_rows_that_end_inside_16_bytes(size, kind, rows):
+    """aligned rows with NaN right behind an end that 16 bytes reach over, in every operand, for small and large tiles: the last step, the only
+    one, the last of a part"""
+    check(*made(*size, kind, rows, seed=19, gap=3))
+
+
 def test_very_many_columns():
     """one sample through more hidden columns than a launch of one wavefront per column could have, and a product as long as that: the columns
     at both ends and the one that the output is made of"""

@@ -11,6 +11,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "../../include/udecore.h"
 
@@ -371,7 +372,8 @@ struct Operand {
     i4 rec[HALVES];
     unsigned step[HALVES];  // bytes of a step
     unsigned off[N];
-    int koff;  // "K": first k of this lane's chunks; "R": not used
+    int koff;           // "K": first k of this lane's chunks; "R": not used
+    int short_at, kleft;  // the step that has only kleft < KS k, or -1
 
     // columns k0.. of rows row0.. of matrices with `rows` rows and K columns
     __device__ inline void init(const void* const* p, const int64_t* ld, int row0, int rows, int k0, int K, int wave, int lane) {
@@ -397,12 +399,19 @@ struct Operand {
             }
         }
     }
-    // the pieces of the whole step n; on = false: zeros, without a trip to memory
+    // the pieces of step n.  END: it may be the short one or lie behind the last (zeros, without a trip to memory)
     unsigned from[HALVES];
     int size[HALVES];
-    __device__ inline void aim(int n, bool on) {
+    template <bool END>
+    __device__ inline void aim(int n, int last) {
+        const bool on = !END || n <= last;
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) from[h] = on ? n * step[h] : 0, size[h] = on ? rec[h][2] : 0;
+        if constexpr (END && KC)
+            if (n == short_at) {  // (chunks behind a row's end.  The rows of an "R" operand behind the last k are behind its records)
+#pragma unroll
+                for (int i = 0; i < N; ++i) off[i] = koff < kleft ? off[i] : OUTSIDE;
+            }
     }
     __device__ inline void piece(int i, unsigned at, int wave) {
         const int h = i / (N / HALVES);
@@ -410,23 +419,15 @@ struct Operand {
         r[2] = size[h];
         to_lds(at + (i * NW + wave) * 1024, off[i], r, from[h]);
     }
-    // a last step of kleft < KS k, `n` steps behind k0; where it ends inside 16 bytes, a "K" operand goes element by element
-    __device__ inline void tail(unsigned at, int wave, int lane, int n, int kleft, char* lds) {
-        if (!KC || kleft % V == 0) {
+    // where a row ends inside 16 bytes: zeros behind its end, in the buffer of that step
+    static __device__ inline void clear(char* lds, int kleft, int tid) {
+        if constexpr (KC) {
+            const int c = kleft / V, e0 = kleft % V;
+            for (int r = tid; r < ROWS; r += 64 * NW) {
+                E* p = (E*)(lds + r * 128 + ((c ^ (r & 7)) << 4));
 #pragma unroll
-            for (int i = 0; i < N; ++i) to_lds(at + (i * NW + wave) * 1024, !KC || koff < kleft ? off[i] : OUTSIDE, rec[i / (N / HALVES)], n * step[i / (N / HALVES)]);
-        } else {
-            typedef E EV __attribute__((ext_vector_type(V)));
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                EV v = {};
-                if (off[i] != OUTSIDE) {
-                    const E* p = (const E*)(base[i / (N / HALVES)] + off[i] + n * step[i / (N / HALVES)]);
-#pragma unroll
-                    for (int e = 0; e < V; ++e)
-                        if (koff + e < kleft) v[e] = p[e];
-                }
-                *(EV*)(lds + (i * NW + wave) * 1024 + lane * 16) = v;
+                for (int e = 1; e < V; ++e)
+                    if (e >= e0) p[e] = 0;
             }
         }
     }
@@ -512,12 +513,12 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
     };
     // (behind the last step: zeros, into buffers that are not read, so that the number of loads on their way is always the same)
     auto load_a = [&](int stage, int n, int last) {
-        oa.aim(n, n <= last);
+        oa.template aim<true>(n, last);
 #pragma unroll
         for (int i = 0; i < OA::N; ++i) oa.piece(i, at + stage, wave);
     };
     auto load_b = [&](int stage, int n, int last) {
-        ob.aim(n, n <= last);
+        ob.template aim<true>(n, last);
 #pragma unroll
         for (int i = 0; i < OB::N; ++i) ob.piece(i, at + stage, wave);
     };
@@ -537,7 +538,19 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
     // of L2, which is what a step of a small tile took with two buffers.  (Without DEEP the loads of a step take about as long to issue as
     // half a step's products: A's third buffer lets the later half of them arrive a step later.)
     constexpr int AHEAD_A = DEEP ? STAGES : 3, AHEAD_B = DEEP ? STAGES : 2, OUT = DEEP ? (STAGES - 2) * (OA::N + OB::N) : OA::N;
-    auto body = [&](int sa, int sa1, int sb, int sb1, int n, int last) {
+    // A last step that is not whole is loaded and multiplied like the others, with zeros behind its end; where that is inside 16 bytes they are
+    // written into LDS once it has arrived.  (As a step of its own behind the loop it cost a trip to memory: 142 instead of 136 us for forward
+    // and pullback of 1000 x 1000 x 2730 in Float16.)  The steps whose loads ahead are whole have a body without those questions: 1 % of
+    // the largest products.
+    int ragged = -1;  // the step that ends inside 16 bytes, or -1
+    auto clear = [&](int sa, int sb) {
+        OA::clear(lds + sa, oa.kleft, tid);
+        OB::clear(lds + sb, oa.kleft, tid);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    // (END: one of the last steps, whose loads ahead may be short or none)
+    auto body = [&](auto end, int sa, int sa1, int sb, int sb1, int n, int last) {
+        constexpr bool END = decltype(end)::value;
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
             reads(i, 1, sa, sb);
@@ -545,10 +558,12 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
             for (int j = 0; j < FN; ++j) acc[i][j] = T::mfma(fb[0][j], fa[0][i], acc[i][j]);
             __builtin_amdgcn_sched_barrier(0);
         }
-        oa.aim(n + AHEAD_A, n + AHEAD_A <= last), ob.aim(n + AHEAD_B, n + AHEAD_B <= last);
+        oa.template aim<END>(n + AHEAD_A, last), ob.template aim<END>(n + AHEAD_B, last);
         __builtin_amdgcn_sched_barrier(0);
         // step n + 1 has arrived (the loads behind it need not have), and nobody reads this step's buffers any more
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(OUT) : "memory");
+        if constexpr (END)
+            if (n + 1 == ragged) clear(sa1, sb1);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
@@ -588,57 +603,54 @@ __global__ __launch_bounds__(64 * NWM * NWN) __attribute__((amdgpu_waves_per_eu(
                 ob.init(pb, lb, n0, q.N, (int)k0, a.K, wave, lane);
             }
             const int left = (int)((kend - k0) / KS), full = left < run ? left : run, rest = left < run ? (int)((kend - k0) % KS) : 0;
-            if (full) {
-                const int last = full - 1;
-                if constexpr (DEEP) {
+            const int steps = full + (rest != 0), last = steps - 1;
+            oa.short_at = ob.short_at = rest ? full : -1, oa.kleft = ob.kleft = rest;
+            ragged = rest % OA::V && (AK || BKc) ? full : -1;
+            if constexpr (DEEP) {
 #pragma unroll
-                    for (int k = 0; k < STAGES; ++k) load_a(k * STAGE, k, last), load_b(k * STAGE + B0, k, last);
-                    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((STAGES - 1) * (OA::N + OB::N)) : "memory");
-                } else {
-                    load_a(A0, 0, last), load_b(0, 0, last);
-                    load_a(A1, 1, last), load_b(OB::BYTES, 1, last);
-                    load_a(A2, 2, last);
-                    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * OA::N + OB::N) : "memory");
-                }
-#pragma unroll
-                for (int j = 0; j < FN; ++j) fb[0][j] = read_b(j, 0, B0);
-#pragma unroll
-                for (int i = 0; i < FM; ++i) fa[0][i] = read_a(i, 0, A0);
-                if constexpr (DEEP) {
-                    int here = 0;
-                    for (int n = 0; n < full; ++n) {
-                        const int next = here + STAGE < STAGES * STAGE ? here + STAGE : 0;
-                        body(here, next, here + B0, next + B0, n, last);
-                        here = next;
-                    }
-                } else {
-                    int s0 = A0, s1 = A1, s2 = A2;
-                    for (int n = 0; n < full; n += 2) {
-                        body(s0, s1, 0, OB::BYTES, n, last);
-                        if (n + 1 < full) body(s1, s2, OB::BYTES, 0, n + 1, last);
-                        const int s = s0;
-                        s0 = s2, s2 = s1, s1 = s;
-                    }
-                }
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                for (int k = 0; k < STAGES; ++k) load_a(k * STAGE, k, last), load_b(k * STAGE + B0, k, last);
+                asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((STAGES - 1) * (OA::N + OB::N)) : "memory");
+            } else {
+                load_a(A0, 0, last), load_b(0, 0, last);
+                load_a(A1, 1, last), load_b(OB::BYTES, 1, last);
+                load_a(A2, 2, last);
+                asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * OA::N + OB::N) : "memory");
             }
-            if (rest) {
-                oa.tail(at + A0, wave, lane, full, rest, lds + A0);
-                ob.tail(at + B0, wave, lane, full, rest, lds + B0);
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (ragged == 0) clear(A0, B0);
 #pragma unroll
-                for (int kk = 0; kk < 2; ++kk) {
+            for (int j = 0; j < FN; ++j) fb[0][j] = read_b(j, 0, B0);
 #pragma unroll
-                    for (int j = 0; j < FN; ++j) fb[0][j] = read_b(j, kk, B0);
-#pragma unroll
-                    for (int i = 0; i < FM; ++i) fa[0][i] = read_a(i, kk, A0);
-#pragma unroll
-                    for (int i = 0; i < FM; ++i)
-#pragma unroll
-                        for (int j = 0; j < FN; ++j) acc[i][j] = T::mfma(fb[0][j], fa[0][i], acc[i][j]);
+            for (int i = 0; i < FM; ++i) fa[0][i] = read_a(i, 0, A0);
+            // (two "R" operands need nothing special at the end; their transposed reads take more registers, which two bodies do not have)
+            constexpr bool APART = AK || BKc;
+            int n = 0;
+            if constexpr (DEEP) {
+                int here = 0;
+                auto step = [&](auto end) {
+                    const int next = here + STAGE < STAGES * STAGE ? here + STAGE : 0;
+                    body(end, here, next, here + B0, next + B0, n, last);
+                    here = next;
+                };
+                if constexpr (APART)
+                    for (; n + AHEAD_A < last; ++n) step(std::false_type());
+                for (; n < steps; ++n) step(std::true_type());
+            } else {
+                int s0 = A0, s1 = A1, s2 = A2;
+                auto turn = [&] {
+                    const int s = s0;
+                    s0 = s2, s2 = s1, s1 = s;
+                };
+                if constexpr (APART)
+                    for (; n + 1 + AHEAD_A < last; n += 2, turn()) {
+                        body(std::false_type(), s0, s1, 0, OB::BYTES, n, last);
+                        body(std::false_type(), s1, s2, OB::BYTES, 0, n + 1, last);
+                    }
+                for (; n < steps; n += 2, turn()) {
+                    body(std::true_type(), s0, s1, 0, OB::BYTES, n, last);
+                    if (n + 1 < steps) body(std::true_type(), s1, s2, OB::BYTES, 0, n + 1, last);
                 }
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             }
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
     }
     if (a.split > 1) {
