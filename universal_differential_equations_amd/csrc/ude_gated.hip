@@ -45,11 +45,11 @@ int vec(const void* p, int64_t ld, int e) { return (uintptr_t)p % 16 == 0 && ld 
 // the start and epilogue of a round, as measured (kernel times over products of 64 x 512 x 1408 to 4096 x 4096 x 11264).
 //   256 x 256: the least that is read again: 4096 x 4096 x 11264 in 271 us = 1395 TFLOP/s; 256 x 128: 311 us; 128 x 128: 365 us.
 //   The smaller ones leave less of the last round idle, but a step costs them 0.25 to 0.5 however little there is in it (LDS, barrier, the
-//   loads' way: 64 x 64 takes 0.25 with its loads four steps ahead, 0.41 with two), so that they are for small products, and for Float32, whose matrix instructions (1/16 of the 16-bit rate) bound it with
+//   loads' way: 64 x 64 takes 0.28 with its loads four steps ahead, 0.41 with two), so that they are for small products, and for Float32, whose matrix instructions (1/16 of the 16-bit rate) bound it with
 //   any tile.
 // EPI_GATE writes ten bytes an element at the end, EPI_PULL reads eight and writes six: with one workgroup on a compute unit nothing is
 // multiplied meanwhile, so that a pull of 4096 x 5632 x 2048 is done in 159 us by 128 x 128 tiles, 171 by 256 x 256 and pieces, 185 by 256 x 128.  Where tiles are few and K is long, K is cut into
-// parts whose sums go through memory (3 TB/s) and one more launch.
+// parts whose sums go through caches and memory (there and back: 5 TB/s, 2.2 past 16 MB) and one more launch (5 us).
 constexpr int CUS = 256;
 constexpr int64_t MOST_PART_BYTES = (int64_t)2 * CUS * 128 * 128 * 4;
 enum { T256 = 0, T256x128 = 1, T128 = 2, T64 = 3, T32 = 4, TILES = 5 };
@@ -64,7 +64,7 @@ constexpr Tile TILE[TILES] = {
     {256, 256, 256, 1, 1, {1.46}, {1.46}, {}, {}, {12, 20, 60}},
     {256, 128, 128, 1, 1, {0.85}, {0.85}, {}, {}, {9, 13, 34}},
     {128, 128, 128, 2, 2, {0.48, 1.02}, {0.48, 1.02}, {1.95, 3.8}, {1.95, 3.8}, {7, 9, 20}},
-    {64, 64, 128, 2, 3, {0.25, 0.43}, {0.40, 0.64}, {0.54, 1.08, 1.6}, {1.08, 2.1, 3.2}, {5, 6, 7}},
+    {64, 64, 128, 2, 3, {0.28, 0.46}, {0.40, 0.64}, {0.54, 1.08, 1.6}, {1.08, 2.1, 3.2}, {5, 6, 7}},
     {32, 128, 128, 3, 3, {0.46, 0.50, 0.65}, {0.46, 0.50, 0.65}, {0.55, 1.1, 1.65}, {0.55, 1.1, 1.65}, {5, 6, 7}}};
 struct Plan {
     int which, split;  // tile; parts of K
@@ -95,7 +95,8 @@ double cut(int which, int epi, int es, int64_t n, int total, int64_t room, int* 
     double least = tiles_cost(which, epi, es, n, total);
     *parts = 1;
     for (int s = 2; s * n <= slots_of(which, es) * CUS && s * n * part_size(which, epi) <= room && s * 2 <= total; ++s) {
-        const double c = tiles_cost(which, epi, es, n * s, (total + s - 1) / s) + n * s * part_size(which, epi) * (2 / 3e6) + 6;
+        const double bytes = (double)(n * s * part_size(which, epi)), far = bytes > 16e6 ? bytes - 16e6 : 0;
+        const double c = tiles_cost(which, epi, es, n * s, (total + s - 1) / s) + bytes / 2.5e6 + far / 2e6 + 5;
         if (c < least) least = c, *parts = s;
     }
     return least;
