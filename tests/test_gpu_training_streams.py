@@ -1,0 +1,110 @@
+"""The training operators on more than one stream and thread: what they keep, what they wait for."""
+import threading
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+
+
+def made(T, D, F, O, kind, seed):
+    gen = torch.Generator().manual_seed(seed)
+    return [(torch.randn(s, generator=gen) * by).to(kind).cuda()
+            for s, by in (((D, T), 1.0), ((F, D), D ** -0.5), ((F, D), D ** -0.5), ((O, F), F ** -0.5), ((T, O), 1.0))]
+
+
+def occupy(n=24):
+    """some milliseconds of work on the current stream"""
+    a = torch.ones((4096, 4096), device="cuda")
+    for _ in range(n):
+        a = (a @ a).mul_(2.0 ** -12)
+    return a
+
+
+def fill_with_nan(shapes, kind):
+    """what the allocator hands out next on the current stream, in the sizes of what a call holds"""
+    return [torch.full(s, float("nan"), dtype=k, device="cuda") for s in shapes for k in (kind, torch.float32) for _ in range(4)]
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("view", [lambda x: x.T, lambda x: x.T.reshape(30, 20, 72), lambda x: x.T[:1].expand(600, -1)], ids=["transposed", "three axes", "broadcast"])
+def test_pullback_on_another_stream_after_saved_is_dropped(view, kind):
+    """x is copied by the forward call, and `saved` is dropped while the other stream has not reached the pullback: the copy's memory, and that
+    of gate and up, is not given to new work of the forward's stream before"""
+    import universal_differential_equations_amd as U
+    T, D, F, O = 600, 72, 104, 40
+    xt, wg, wu, wd, dy = made(T, D, F, O, kind, 21)
+    x = view(xt)
+    dy = dy.view(*x.shape[:-1], O)
+    want = U.gated_ffn_pullback(U.gated_ffn(x, wg, wu, wd, save=True)[1], dy)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        saved = U.gated_ffn(x, wg, wu, wd, save=True)[1]
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            occupy()
+            got = U.gated_ffn_pullback(saved, dy)
+        del saved
+        held = fill_with_nan([(T, D), (2, T, F)], kind)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        del held, got
+
+
+def test_pullbacks_in_threads_that_hold_the_last_reference():
+    """each thread takes its `saved` out of a list, so that its own reference is the last one; every comparison is counted, every error kept"""
+    import universal_differential_equations_amd as U
+    T, D, F, O = 90, 72, 104, 40
+    sets = [made(T, D, F, O, torch.float32, s) for s in (22, 23)]
+    want = [U.gated_ffn_pullback(U.gated_ffn(s[0].T, *s[1:4], save=True)[1], s[4]) for s in sets]
+    torch.cuda.synchronize()
+    good, bad = [], []
+
+    def go(i, box, ready):
+        try:
+            stream = torch.cuda.Stream()
+            stream.wait_event(ready)
+            with torch.cuda.stream(stream):
+                occupy(4)
+                got = U.gated_ffn_pullback(box.pop(), sets[i][4])
+                stream.synchronize()
+            (good if all(torch.equal(a, b) for a, b in zip(got, want[i])) else bad).append(i)
+        except Exception as e:  # (an error in a thread would otherwise be lost)
+            bad.append(e)
+
+    for _ in range(5):
+        ts = []
+        for i in (0, 1):
+            box = [U.gated_ffn(sets[i][0].T, *sets[i][1:4], save=True)[1]]
+            ready = torch.cuda.Event()
+            ready.record()
+            ts.append(threading.Thread(target=go, args=(i, box, ready)))
+            del box
+        [t.start() for t in ts]
+        for _ in range(5):
+            fill_with_nan([(T, D), (2, T, F)], torch.float32)
+        [t.join() for t in ts]
+    assert not bad and len(good) == 10
+
+
+def test_forward_calls_of_two_threads_are_all_compared():
+    import universal_differential_equations_amd as U
+    sets = [made(90, 72, 104, 40, torch.float32, s) for s in (24, 25)]
+    want = [U.gated_ffn(s[0].T, *s[1:4]) for s in sets]
+    torch.cuda.synchronize()
+    good, bad = [], []
+
+    def go(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    (good if torch.equal(U.gated_ffn(sets[i][0].T, *sets[i][1:4]), want[i]) else bad).append(i)
+        except Exception as e:
+            bad.append(e)
+
+    ts = [threading.Thread(target=go, args=(i,)) for i in (0, 1)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert not bad and len(good) == 40

@@ -96,9 +96,13 @@ class _Block:
         """this thread's context, on the current stream"""
         eng, stream = self.eng, current_raw_stream(self.device.index)
         eng.set_stream(stream)
-        if stream != self.stream and self.gate is not None:
-            # (saved on the forward call's stream: its memory is not given away before this one is done with it)
-            self.gate.record_stream(self.torch.cuda.current_stream(self.device))
+        if stream != self.stream:
+            # held since the forward call, on its stream; of x's copy (see _rows) and of gate and up nobody else has a reference: the memory is not
+            # given away before this stream is done with it
+            now = self.torch.cuda.current_stream(self.device)
+            for t in (self.x, *self.w, self.gate):
+                if t is not None:
+                    t.record_stream(now)
         return eng
 
 
