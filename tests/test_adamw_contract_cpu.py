@@ -1,0 +1,84 @@
+"""What an AdamW step takes, refuses and counts: the host's part of it, on CPU tensors with the launch replaced by a record; no GPU."""
+import ctypes as C
+import types
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture
+def training(monkeypatch):
+    """the module, whose device checks take CPU tensors and whose launches append what they are given to `training.launched`: one dict of
+    (grad as floats in the parameter's order, n) per tensor, and the step number"""
+    from universal_differential_equations_amd import _lib, training
+    launched = []
+
+    def launch(handle, o, n, table):
+        grads = []
+        for i in range(n):
+            t = table[i]
+            grads.append(list((C.c_float * t.n).from_address(t.grad)) if t.n else None)
+        launched.append(types.SimpleNamespace(step=o._obj.step, step_dev=o._obj.step_dev, grads=grads))
+        return 0
+
+    def check(rc):
+        assert rc == 0
+
+    eng = types.SimpleNamespace(h=None, check=check, L=types.SimpleNamespace(ude_adamw_step_dev=launch))
+    monkeypatch.setattr(training, "_device_list", lambda what, ts: (ts[0].device, str(ts[0].dtype)[6:]))
+    monkeypatch.setattr(training, "_bound_engine", lambda dev: eng)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(training, "launched", launched, raising=False)
+    assert _lib.ADAMW_BLOCK == 256
+    return training
+
+
+def test_a_gradient_of_another_shape_is_refused(training):
+    """as many elements in another order: (D, F) parameters and the (F, D) gradient of their transpose"""
+    p, q = torch.zeros(3, 5), torch.zeros(4)
+    opt = training.AdamW([p, q])
+    for bad in ((5, 3), (15,), (15, 1), (1, 3, 5)):
+        with pytest.raises(ValueError, match="gradient 0"):
+            opt.step([torch.ones(bad), torch.ones(4)])
+        with pytest.raises(ValueError, match="gradient 0"):
+            opt.step([torch.ones(bad), None])
+    with pytest.raises(ValueError, match="gradient 1"):
+        opt.step([None, torch.ones(2, 2)])
+    assert opt.steps == 0 and not training.launched
+
+
+def test_a_gradient_of_another_stride_order_is_taken_element_by_element(training):
+    p = torch.zeros(3, 5)
+    opt = training.AdamW([p])
+    g = torch.arange(15.0).reshape(5, 3).T    # (3, 5), columns adjacent: what a pullback by columns hands back
+    opt.step([g])
+    opt.step([g.contiguous()])
+    opt.step([None])
+    assert [x.grads[0] for x in training.launched] == [g.reshape(-1).tolist()] * 2 + [None]
+    assert [x.step for x in training.launched] == [1, 2, 3] and opt.steps == 3
+
+
+def test_a_reshaped_or_transposed_parameter(training):
+    """other views of the same storage, which starts where it did"""
+    p = torch.zeros(3, 5)
+    opt = training.AdamW([p])
+    p.data = p.data.view(5, 3)
+    opt.step([torch.ones(5, 3)])
+    opt.step([torch.ones(5, 3)])
+    with pytest.raises(ValueError, match="gradient 0"):
+        opt.step([torch.ones(3, 5)])
+    p.data = torch.zeros(4, 4)
+    with pytest.raises(ValueError, match="parameter 0"):
+        opt.step([torch.ones(4, 4)])
+    p = torch.zeros(12)
+    opt = training.AdamW([p])
+    p.data = p.data[:4]   # (starts where it did, and is shorter than the moments)
+    with pytest.raises(ValueError, match="parameter 0"):
+        opt.step([torch.ones(4)])
+    q = torch.zeros(4, 4)
+    opt = training.AdamW([q])
+    q.data = q.data.T
+    with pytest.raises(ValueError, match="parameter 0"):
+        opt.step([torch.ones(4, 4)])
+    assert opt.steps == 0

@@ -144,7 +144,7 @@ class AdamW:
             t.m_scale, t.v_scale = (s[k].data_ptr() if k in s else None for k in ("m_scale", "v_scale"))
             t.param, t.n, t.weight_decay = p.data_ptr(), p.numel(), decay[i]
             self._live[i] = p.numel()
-        self._at = [p.data_ptr() for p in self.params]
+        self._at, self._shapes = [p.data_ptr() for p in self.params], [p.shape for p in self.params]
         self._opts = _lib.AdamwOpts(param_dtype=_lib.DTYPE_CODE[self.dtype], state_bits=bits)
 
     def _make_state(self, i, master, given):
@@ -176,22 +176,25 @@ class AdamW:
         return [dict(s) for s in self._state]
 
     def step(self, grads, clip=None):
-        """one update with `grads` (a tensor per parameter, of the parameters' dtype or, for 16-bit parameters, float32; None: that
-        parameter and its moments stay as they are); clip: `grad_norm(...)`'s result, whose factor scales the gradients"""
+        """one update with `grads` (a tensor per parameter, of its shape and of the parameters' dtype or, for 16-bit parameters, float32; any
+        strides; None: that parameter and its moments stay as they are); clip: `grad_norm(...)`'s result, whose factor scales the gradients.
+        Parameters that a block holds by columns (w = s.T) are given as the storage s, their gradients as g.T"""
         torch, table = self.torch, self._table
         if len(grads) != len(self.params):
             raise ValueError("AdamW: %d gradients for %d parameters" % (len(grads), len(self.params)))
         at = [p.data_ptr() for p in self.params]
-        if at != self._at:
+        if at != self._at or not all([p.is_contiguous() for p in self.params]):
             self._moved(at)
         have = [g for g in grads if g is not None]
-        sizes = self._live if len(have) == len(grads) else [k for k, g in zip(self._live, grads) if g is not None]
+        shapes = self._shapes if len(have) == len(grads) else [s for s, g in zip(self._shapes, grads) if g is not None]
         dts = {g.dtype for g in have}
-        if len(dts) > 1 or [g.numel() for g in have] != sizes or {g.get_device() for g in have} - {self.device.index}:
-            for i, (g, k) in enumerate(zip(grads, self._live)):
-                if g is not None and (g.dtype != have[0].dtype or g.numel() != k or g.device != self.device):
-                    raise ValueError("AdamW: gradient %d is %s of %d elements on %s; %s of %d on %s is needed"
-                                     % (i, g.dtype, g.numel(), g.device, have[0].dtype, k, self.device))
+        # (of the same shape, not of as many elements: the transposed gradient would be applied to other elements)
+        if len(dts) > 1 or [g.shape for g in have] != shapes or {g.get_device() for g in have} - {self.device.index}:
+            self._moved(at)
+            for i, (g, p) in enumerate(zip(grads, self.params)):
+                if g is not None and (g.dtype != have[0].dtype or g.shape != p.shape or g.device != self.device):
+                    raise ValueError("AdamW: gradient %d is %s %s on %s; %s %s on %s is needed"
+                                     % (i, g.dtype, tuple(g.shape), g.device, have[0].dtype, tuple(p.shape), self.device))
         if not all([g.is_contiguous() for g in have]):
             grads = [g if g is None else g.contiguous() for g in grads]   # (kept until the launch)
         if len(have) == len(grads):
@@ -221,12 +224,12 @@ class AdamW:
         self.steps += 1
 
     def _moved(self, at):
-        """parameters were given other storage"""
+        """parameters were given other storage, or another layout of theirs"""
         for i, p in enumerate(self.params):
             if p.device != self.device or str(p.dtype)[6:] != self.dtype or p.numel() != self._live[i] or not p.is_contiguous():
-                raise ValueError("AdamW: parameter %d was replaced by %s of %d elements on %s" % (i, p.dtype, p.numel(), p.device))
+                raise ValueError("AdamW: parameter %d was replaced by %s of %d elements on %s (strides %s)" % (i, p.dtype, p.numel(), p.device, p.stride()))
         self._columns[:, 0] = at
-        self._at = at
+        self._at, self._shapes = at, [p.shape for p in self.params]
 
     def moments(self, out=None):
         """[(m, v), ...]: the values of the moments, Float32 (Float64 for float64 parameters); out: pairs of tensors to write 8-bit
