@@ -82,3 +82,41 @@ def test_a_reshaped_or_transposed_parameter(training):
     with pytest.raises(ValueError, match="parameter 0"):
         opt.step([torch.ones(4, 4)])
     assert opt.steps == 0
+
+
+def test_steps_counted_on_the_device_are_the_steps(training, monkeypatch):
+    """capturable=True: a replayed graph counts in `count` alone, and `steps` is what another instance continues from"""
+    p = torch.zeros(6)
+    opt = training.AdamW([p], capturable=True, step=4)
+    assert opt.steps == 4
+    opt.step([torch.ones(6)])
+    assert opt.steps == 5 and int(opt.count) == 5 and training.launched[-1].step_dev == opt.count.data_ptr()
+    opt.count.add_(1000)   # (what replays do)
+    assert opt.steps == 1005
+    two = training.AdamW([torch.zeros(6)], step=opt.steps)
+    two.step([torch.ones(6)])
+    assert training.launched[-1].step == 1006 and two.steps == 1006
+    opt.steps = 7
+    assert opt.steps == 7 and int(opt.count) == 7
+    two.steps = 7
+    two.step([torch.ones(6)])
+    assert training.launched[-1].step == 8 and two.steps == 8 and two.count is None
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(ValueError, match="captur"):
+        opt.steps
+
+
+def test_a_refused_launch_is_not_counted(training):
+    from universal_differential_equations_amd import UdeError
+
+    def check(rc):
+        if rc:
+            raise UdeError(rc, "refused")
+
+    eng = training._bound_engine(None)
+    eng.check, eng.L.ude_adamw_step_dev = check, lambda *a: -1
+    for capturable in (True, False):
+        opt = training.AdamW([torch.zeros(6)], capturable=capturable)
+        with pytest.raises(UdeError):
+            opt.step([torch.ones(6)])
+        assert opt.steps == 0

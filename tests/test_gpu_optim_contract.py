@@ -44,3 +44,34 @@ def test_weights_by_columns_through_block_and_step():
     again = [b.clone() for b in before]
     training.AdamW(again, **HYPER).step([g.contiguous().T for g in grads])
     assert all(torch.equal(a, s) for a, s in zip(again, stores))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_resumed_after_replays(bits):
+    """a checkpoint (state, steps) taken after a graph was replayed goes on like the instance that was never captured"""
+    from universal_differential_equations_amd import training
+    gen = torch.Generator().manual_seed(32)
+    start, g = (torch.randn(700, generator=gen).cuda() for _ in range(2))
+    eager, held = start.clone(), start.clone()
+    one = training.AdamW([eager], bits=bits, **HYPER)
+    two = training.AdamW([held], bits=bits, capturable=True, **HYPER)
+    one.step([g]), two.step([g])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        two.step([g])
+        with pytest.raises(ValueError, match="captur"):
+            two.steps
+    assert two.steps == 1   # (captured, not run)
+    for i in range(40):
+        graph.replay()
+        one.step([g])
+        assert i % 13 or two.steps == i + 2
+    assert one.steps == two.steps == 41
+    copies = [held.clone()]
+    three = training.AdamW(copies, bits=bits, state=[{k: x.clone() for k, x in two.state[0].items()}], step=two.steps, **HYPER)
+    three.step([g]), one.step([g])
+    # (bias corrections of the device's pow() are at most one unit in the last place of Float64 off the host's: the same Float32 factors but for
+    # a value next to a border, and then a step's last place: 42 steps of at most eta and two places each)
+    assert three.steps == one.steps == 42
+    assert float((copies[0] - eager).abs().max()) <= 42 * 0.01 * 2 * 2.0 ** -23 + 4 * 2.0 ** -24 * float(eager.abs().max())

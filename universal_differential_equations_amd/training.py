@@ -103,7 +103,8 @@ class AdamW:
     codes with two scales per 256 elements (ude_adamw_tensor).  master=True keeps a Float32 copy of 16-bit parameters that the updates
     accumulate in.  state: one dict per tensor with "m", "v" (codes: int8, uint8, with "m_scale", "v_scale") and "master" -- tensors that
     are used as they are, e.g. another instance's `state` out of a checkpoint; step: the steps already done.  capturable=True counts
-    the steps on the device, as a step that is captured into a hipGraph needs.  skip_nonfinite=True leaves everything as it was in a step
+    the steps on the device (`count`, which `steps` reads), as a step that is captured into a hipGraph needs; eta, beta, eps and decay are those of the
+    capture.  skip_nonfinite=True leaves everything as it was in a step
     whose clip[0] is not finite (the step is counted).  A non-finite gradient makes the 8-bit moments of its block of 256 NaN."""
 
     def __init__(self, params, eta=0.001, beta=(0.9, 0.999), eps=1e-8, weight_decay=0.01, bits=32, master=False, state=None, step=0,
@@ -124,9 +125,9 @@ class AdamW:
         decay = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
         if len(decay) != n:
             raise ValueError("AdamW: %d values of weight_decay for %d parameters" % (len(decay), n))
-        self.eta, self.beta, self.eps, self.bits, self.steps = eta, tuple(beta), eps, bits, int(step)
+        self.eta, self.beta, self.eps, self.bits, self._steps = eta, tuple(beta), eps, bits, int(step)
         self.skip_nonfinite = bool(skip_nonfinite)
-        self.count = torch.full((1,), self.steps, dtype=torch.int64, device=self.device) if capturable else None
+        self.count = torch.full((1,), self._steps, dtype=torch.int64, device=self.device) if capturable else None
         if state is not None and len(state) != n:
             raise ValueError("AdamW: state of %d tensors for %d parameters" % (len(state), n))
         self._state = [self._make_state(i, master, None if state is None else state[i]) for i in range(n)]
@@ -175,6 +176,23 @@ class AdamW:
         """one dict of tensors per parameter (the tensors themselves: copy into them to change the state)"""
         return [dict(s) for s in self._state]
 
+    @property
+    def steps(self):
+        """the steps done: with `state`, what another instance continues from (step=).  capturable=True: read from the device, where replays count
+        (waits for the current stream; refused while that is captured)"""
+        if self.count is None:
+            return self._steps
+        if self.torch.cuda.is_current_stream_capturing():
+            raise ValueError("AdamW: steps are counted on the device, and cannot be read while a graph is captured")
+        return int(self.count.item())
+
+    @steps.setter
+    def steps(self, n):
+        if self.count is None:
+            self._steps = int(n)
+        else:
+            self.count.fill_(int(n))
+
     def step(self, grads, clip=None):
         """one update with `grads` (a tensor per parameter, of its shape and of the parameters' dtype or, for 16-bit parameters, float32; any
         strides; None: that parameter and its moments stay as they are); clip: `grad_norm(...)`'s result, whose factor scales the gradients.
@@ -216,12 +234,13 @@ class AdamW:
             o.step_dev = self.count.data_ptr()
         elif torch.cuda.is_current_stream_capturing():
             raise ValueError("AdamW: a step that is captured into a graph has to count on the device: capturable=True")
-        o.step = self.steps + 1
+        o.step = self._steps + 1   # (not read where step_dev is given)
         rc = eng.L.ude_adamw_step_dev(eng.h, C.byref(o), len(table), table)
         if rc and self.count is not None:
             self.count.sub_(1)
         eng.check(rc)
-        self.steps += 1
+        if self.count is None:
+            self._steps += 1
 
     def _moved(self, at):
         """parameters were given other storage, or another layout of theirs"""
