@@ -120,3 +120,15 @@ def test_a_refused_launch_is_not_counted(training):
         with pytest.raises(UdeError):
             opt.step([torch.ones(6)])
         assert opt.steps == 0
+
+
+def test_parameter_arrays_of_the_deep_bsde_networks():
+    """their lengths, in the order of the flat vector: a glorot-uniform weight (no zero but by chance) and a zero bias in turn"""
+    import numpy as np
+    from universal_differential_equations_amd import pde
+    for d, hls in ((100, 110), (3, 7), (1, 1)):
+        nets = pde.NNPDENS(d, hls)
+        sizes, theta = nets.array_sizes(), nets.init_params(np.random.default_rng(0))
+        assert len(sizes) == 14 and sum(sizes) == theta.size == sum(nets.num_params()) and sum(sizes[:6]) == nets.num_params()[0]
+        for i, part in enumerate(np.split(theta, np.cumsum(sizes)[:-1])):
+            assert part.any() == (i % 2 == 0)

@@ -75,3 +75,49 @@ def test_resumed_after_replays(bits):
     # value next to a border.  Then each of 42 steps, of at most 2 eta with 8-bit moments, is two places off, and the parameter rounded otherwise
     assert three.steps == one.steps == 42
     assert float((copies[0] - eager).abs().max()) <= 42 * 2.0 ** -23 * (4 * 0.01 + float(eager.abs().max()))
+
+
+def test_deep_bsde_steps_are_flux_adamw_behind_clipnorm():
+    """pde.solve with ADAMW(eta, beta, decay, max_norm) against Optimiser(ClipNorm, ADAMW) in Float64: every parameter array is scaled by its own
+    norm, then theta <- theta - eta m^ / (sqrt(v^) + eps) - decay theta; each step from the device's own theta and gradient"""
+    from universal_differential_equations_amd import pde
+    prob = pde.TerminalPDEProblem(pde.hjb(1.0), np.zeros(100, dtype=np.float32), (0.0, 1.0))
+    nets = pde.NNPDENS(100, 110)
+    th0 = nets.init_params(np.random.default_rng(1))
+    kw = dict(alg=pde.LambaEM(), abstol=0.1, reltol=0.1)
+    dims = [n for net in ((100, 110, 110, 1), (101, 110, 110, 110, 100)) for i, o in zip(net, net[1:]) for n in (i * o, o)]
+    bs = pde.DeviceBSDE(prob, nets, kw["alg"], 32, abstol=0.1, reltol=0.1)
+    theta = torch.tensor(th0, device="cuda")
+    assert sum(dims) == theta.numel() == bs.np
+
+    def norms(g):
+        return [float(x.double().norm()) for x in g.split(dims)]
+
+    first = norms(bs.loss_grad(theta, it=0)[1])
+    most = sorted(x for x in first if x > 0)[len(first) // 2]     # some arrays are over it and some not
+    eta, beta, decay = 0.02, (0.9, 0.99), 0.003
+    opt = pde.ADAMW(eta, beta=beta, decay=decay, max_norm=most)
+    m = {k: torch.zeros(theta.numel(), dtype=torch.float64, device="cuda") for k in ("each", "all")}
+    v, terms = ({k: x.clone() for k, x in m.items()} for _ in range(2))
+    for t in (1, 2, 3):
+        g = bs.loss_grad(theta, it=t - 1)[1].clone()
+        n = norms(g)
+        factors = {"each": [min(1.0, most / x) if x else 1.0 for x in n], "all": [min(1.0, most / math.sqrt(sum(x * x for x in n)))] * len(n)}
+        after = pde.solve(prob, pde.NNPDENS(100, 110, opt=opt), th0, maxiters=t, trajectories=32, pabstol=1e-9, **kw)[1]
+        off = {}
+        for k, fs in factors.items():
+            gs = g.double() * torch.tensor(np.repeat(fs, dims), device="cuda")
+            m[k], v[k] = beta[0] * m[k] + (1 - beta[0]) * gs, beta[1] * v[k] + (1 - beta[1]) * gs * gs
+            terms[k] = beta[0] * terms[k] + (1 - beta[0]) * gs.abs()
+            under = (v[k] / (1 - beta[1] ** t)).sqrt() + 1e-8
+            want = theta.double() * (1 - decay) - eta * (m[k] / (1 - beta[0] ** t)) / under
+            # Roundings of 2^-24, moments carried in Float32: m's two products, its sum and the casts of factor and beta, 5 a step of the terms
+            # that it is made of (which may cancel), 15 after three; v's 6 a step, all terms positive, 18 halved by the root; root, eps,
+            # quotient, product, two bias corrections, the scaled gradient: 7.  31 of the step's terms, rounded up to 40; 3 of the parameter.
+            # What is subnormal in Float32, over eps: below 2^-100
+            size = eta * (terms[k] / (1 - beta[0] ** t)) / under
+            bound = 40 * U24 * size + 3 * U24 * theta.double().abs() + 2.0 ** -100
+            off[k] = float(((after.double() - want).abs() / bound).max())
+        assert off["each"] <= 1, (t, off)
+        theta = after
+    assert off["all"] > 10 and min(first) < most < max(first)   # (one norm of all arrays would have been seen)

@@ -59,8 +59,8 @@ class ADAM:
 
 class ADAMW:
     """Flux.ADAMW(eta, (0.9, 0.999), decay) = Optimiser(ADAM(eta, beta), WeightDecay(decay)): the update of ADAM plus decay * theta, with,
-    where max_norm is given, ClipNorm(max_norm) in front of it.  The step and the norm are single launches over the parameters in HBM
-    (training.AdamW, training.grad_norm)."""
+    where max_norm is given, ClipNorm(max_norm) in front of it, which scales each parameter array's gradient by that array's own norm.  The
+    step is one launch over the parameters in HBM, each norm another (training.AdamW, training.grad_norm)."""
 
     def __init__(self, eta=0.001, beta=(0.9, 0.999), decay=0.0, max_norm=None):
         if not eta > 0:
@@ -74,6 +74,11 @@ class NNPDENS:
 
     def __init__(self, d, hls, opt=None):
         self.d, self.hls, self.opt = d, hls, opt or ADAM(0.001)
+
+    def array_sizes(self):
+        """elements of the arrays of Flux.params(u0, sigma^T grad u), in their order: W and b of each layer"""
+        d, h = self.d, self.hls
+        return [n for net in ((d, h, h, 1), (d + 1, h, h, h, d)) for fin, fout in zip(net, net[1:]) for n in (fin * fout, fout)]
 
     def num_params(self):
         a, b = C.c_int32(0), C.c_int32(0)
@@ -209,7 +214,10 @@ def solve(prob, pdealg, theta0, verbose=False, maxiters=300, trajectories=100, a
         if lval < pabstol:
             break
         if fused is not None:
-            fused.step([g], clip=None if opt.max_norm is None else training.grad_norm([g], opt.max_norm))
+            if opt.max_norm is not None:   # (Flux applies an optimiser to one parameter array at a time: ClipNorm knows no norm of them all)
+                for part in g.split(pdealg.array_sizes()):
+                    part.mul_(training.grad_norm([part], opt.max_norm)[1])
+            fused.step([g])
             continue
         # Flux.ADAM (0.9): mt = b1 mt + (1-b1) g; vt = b2 vt + (1-b2) g^2; theta -= mt/(1-b1^t) / (sqrt(vt/(1-b2^t)) + eps) * eta
         m.mul_(opt.beta[0]).add_(g, alpha=1 - opt.beta[0])
