@@ -152,6 +152,10 @@ const char* ude_last_error(ude_ctx* ctx);
  * workspaces grow -- a larger ensemble, an automatic dense-store regrowth after UDE_RET_DENSE_OVERFLOW) and do not run ordinary calls of
  * the same context on another stream concurrently with a replay: the library keeps no ordering between them. */
 int ude_set_stream(ude_ctx* ctx, void* hip_stream);
+/* stream of the training operators (ude_gated_ffn_*_dev, ude_adamw_*_dev, ude_grad_norm_dev) alone, until the next ude_set_stream: they use no
+ * memory of the context, so that nothing waits for anything -- work of the context on its own stream goes on beside them, and what
+ * order they need among each other is the caller's to give. */
+int ude_set_operator_stream(ude_ctx* ctx, void* hip_stream);
 int ude_set_launch_opts(ude_ctx* ctx, const ude_launch_opts* lo);
 /* 0: this (model, alg) runs on a compiled fast instance; 1: it runs on a runtime-shape fallback kernel -- any chain of <= 8 Dense
  * layers of width <= 64, activations identity / tanh / rbf / relu, for UDE_KIND_LV_UDE 2 -> 2 (Float64 and Float32),
@@ -332,7 +336,7 @@ int ude_last_kernel_ms(ude_ctx* ctx, float* fwd_ms, float* bwd_ms);
  * Training operators on device buffers: a gated feed-forward block with its pullback, the AdamW step over many tensors, the global
  * gradient norm.  They replace nothing of the reference's scripts (their networks are Dense chains and their optimiser is ADAM:
  * scenario_1.jl:62-64,111; highdim_pde/lambaem.jl:23-31): they are the layer and the optimiser step of larger networks, next to them.
- * Every call enqueues on the context's stream, may be captured into a hipGraph and uses no memory but its arguments: the caller owns
+ * Every call enqueues on the context's stream (or ude_set_operator_stream's), may be captured into a hipGraph and uses no memory but its arguments: the caller owns
  * the workspace (its contents need not be kept between calls; calls that may run at the same time -- two streams, two captured graphs
  * -- need one each).  Sizes and host-side arguments are baked into a captured call. */
 enum { UDE_DT_F64 = 0, UDE_DT_F32 = 1, UDE_DT_F16 = 2, UDE_DT_BF16 = 3 };

@@ -100,7 +100,7 @@ EXPORTS = ["ude_version", "ude_create", "ude_destroy", "ude_last_error", "ude_se
            "ude_allreduce_grad_local", "ude_allreduce_grad_p2p", "ude_comm_create_p2p", "ude_comm_p2p_connect",
            "ude_allreduce_grad_p2p_mp", "ude_comm_p2p_status", "ude_comm_p2p_disconnect", "ude_pack_counters_dev",
            "ude_gated_ffn_workspace", "ude_gated_ffn_forward_dev", "ude_gated_ffn_backward_dev", "ude_adamw_step_dev",
-           "ude_adamw_moments_dev", "ude_grad_norm_workspace", "ude_grad_norm_dev"]
+           "ude_adamw_moments_dev", "ude_grad_norm_workspace", "ude_grad_norm_dev", "ude_set_operator_stream"]
 
 
 def load():
@@ -128,6 +128,7 @@ def load():
     L.ude_last_error.argtypes = [vp]
     L.ude_last_error.restype = C.c_char_p
     L.ude_set_stream.argtypes = [vp, vp]
+    L.ude_set_operator_stream.argtypes = [vp, vp]
     L.ude_set_launch_opts.argtypes = [vp, C.POINTER(LaunchOpts)]
     L.ude_model_supported.argtypes = [vp, C.POINTER(ModelDesc), C.POINTER(SolveOpts), i32]
     common = [vp, C.POINTER(ModelDesc), C.POINTER(SolveOpts), i64, vp, vp, vp, vp, i32]

@@ -25,6 +25,10 @@ struct ude_ctx {
     int64_t prev_cost_n = 0;     // cost-ordered launch: prev_cost holds the backward step attempts of the last such call (N members, signature below)
     int64_t prev_cost_sig = 0;
     hipEvent_t ev_sync = nullptr;  // orders work across a change of the bound stream
+    // the training operators' stream: they use no workspace of the context, and are ordered with none of its work
+    hipStream_t op_stream = nullptr;
+    bool op_bound = false;
+    hipStream_t operators() const { return op_bound ? op_stream : stream; }
     int ncu = 0;         // compute units of the device (queried once)
     int auto_cap = 256;  // dense-store capacity used when lo.max_dense_steps == 0; grows x4 on DenseOverflow (host-buffer path)
     int64_t trace_traj = -1;

@@ -160,7 +160,7 @@ int launch3(ude_ctx* c, Args a, bool tile) {
     if constexpr (EPI != EPI_PULL && AK && BKc) {
         if (few(a, EPI, sizeof(typename T::E), tile)) {
             const int M = a.p[0].M;
-            auto go = [&](auto kernel, int columns) { hipLaunchKernelGGL(kernel, dim3((unsigned)((a.p[0].N + 4 * columns - 1) / (4 * columns))), dim3(256), 0, c->stream, a); };
+            auto go = [&](auto kernel, int columns) { hipLaunchKernelGGL(kernel, dim3((unsigned)((a.p[0].N + 4 * columns - 1) / (4 * columns))), dim3(256), 0, c->operators(), a); };
             if (M == 1) go(few_rows<T, EPI, 1>, Few<EPI, 1>::NT);
             else if (M == 2) go(few_rows<T, EPI, 2>, Few<EPI, 2>::NT);
             else go(few_rows<T, EPI, 4>, Few<EPI, 4>::NT);
@@ -172,7 +172,7 @@ int launch3(ude_ctx* c, Args a, bool tile) {
     if (tile && p.big * p.split < 1 << 22 && p.all < 1 << 22) {
         constexpr bool GATE = EPI == EPI_GATE, HALF = sizeof(typename T::E) == 2;
         const dim3 block(256);
-        auto go = [&](auto kernel, dim3 g) { hipLaunchKernelGGL(kernel, g, block, 0, c->stream, a); };
+        auto go = [&](auto kernel, dim3 g) { hipLaunchKernelGGL(kernel, g, block, 0, c->operators(), a); };
         // `tiles` of a kind, each cut into `split` parts
         auto run = [&](int which, int64_t tiles, int split) {
             a.split = split, a.tiles = (int)tiles;
@@ -209,7 +209,7 @@ int launch3(ude_ctx* c, Args a, bool tile) {
         n = t > n ? t : n;
     }
     if (n >= 1 << 24) return fail(c, UDE_ERR_UNSUPPORTED, "gated_ffn: %lld tiles", (long long)n);
-    hipLaunchKernelGGL((gemm_any<T, EPI, AK, BKc>), dim3((unsigned)n, 1, a.nprod), dim3(256), 0, c->stream, a);
+    hipLaunchKernelGGL((gemm_any<T, EPI, AK, BKc>), dim3((unsigned)n, 1, a.nprod), dim3(256), 0, c->operators(), a);
     HIPCHK(c, hipGetLastError());
     return UDE_OK;
 }

@@ -523,9 +523,9 @@ int check_state(ude_ctx* c, const ude_adamw_tensor& t, int64_t i, int bits, int 
 template <class P, class G>
 void adam_launch(ude_ctx* c, const AdamArgs& a, int bits, unsigned chunks) {
     if (bits == 8) {
-        if constexpr (sizeof(typename P::W) == 4) hipLaunchKernelGGL((adamw8_kernel<P, G>), dim3(chunks), dim3(256), 0, c->stream, a);
+        if constexpr (sizeof(typename P::W) == 4) hipLaunchKernelGGL((adamw8_kernel<P, G>), dim3(chunks), dim3(256), 0, c->operators(), a);
     } else {
-        hipLaunchKernelGGL((adamw32_kernel<P, G>), dim3(chunks), dim3(256), 0, c->stream, a);
+        hipLaunchKernelGGL((adamw32_kernel<P, G>), dim3(chunks), dim3(256), 0, c->operators(), a);
     }
 }
 
@@ -624,7 +624,7 @@ extern "C" int ude_adamw_moments_dev(ude_ctx* c, int64_t nt, const ude_adamw_ten
         [&](int slot, int64_t i) { a.t[slot] = {(const int8_t*)ts[i].m, (const uint8_t*)ts[i].v, ts[i].m_scale, ts[i].v_scale, m_out[i], v_out[i], ts[i].n}; },
         [&](int used, int64_t chunks) {
             a.nt = used;
-            hipLaunchKernelGGL(moments_kernel, dim3((unsigned)chunks), dim3(256), 0, c->stream, a);
+            hipLaunchKernelGGL(moments_kernel, dim3((unsigned)chunks), dim3(256), 0, c->operators(), a);
             HIPCHK(c, hipGetLastError());
             return (int)UDE_OK;
         });
@@ -664,12 +664,12 @@ extern "C" int ude_grad_norm_dev(ude_ctx* c, int32_t dtype, int64_t nt, const vo
     auto run = [&](auto g, int64_t chunks) {
         typedef decltype(g) G;
         if (sums == 0 && chunks <= NORM_ONE && need <= 8 * chunks) {  // (they are all there are)
-            hipLaunchKernelGGL((norm_one_kernel<G>), dim3(1), dim3(1024), 0, c->stream, a, max_norm, out);
+            hipLaunchKernelGGL((norm_one_kernel<G>), dim3(1), dim3(1024), 0, c->operators(), a, max_norm, out);
             done = true;
             return;
         }
         const unsigned blocks = (unsigned)(chunks < NORM_BLOCKS ? chunks : NORM_BLOCKS);
-        hipLaunchKernelGGL((norm_part_kernel<G>), dim3(blocks), dim3(256), 0, c->stream, a);
+        hipLaunchKernelGGL((norm_part_kernel<G>), dim3(blocks), dim3(256), 0, c->operators(), a);
         sums += blocks;
     };
     const int rc = in_launches(
@@ -691,7 +691,7 @@ extern "C" int ude_grad_norm_dev(ude_ctx* c, int32_t dtype, int64_t nt, const vo
             return (int)UDE_OK;
         });
     if (rc || done) return rc;
-    hipLaunchKernelGGL(norm_join_kernel, dim3(1), dim3(256), 0, c->stream, (const double*)ws, (int)sums, max_norm, out);
+    hipLaunchKernelGGL(norm_join_kernel, dim3(1), dim3(256), 0, c->operators(), (const double*)ws, (int)sums, max_norm, out);
     HIPCHK(c, hipGetLastError());
     return UDE_OK;
 }

@@ -782,6 +782,7 @@ static bool capturing(hipStream_t st) {
 extern "C" int ude_set_stream(ude_ctx* c, void* s) {
     if (!c) return UDE_ERR_INVALID;
     hipStream_t ns = (hipStream_t)s;
+    c->op_bound = false;
     if (ns != c->stream) {
         // the workspaces are shared by every call on this context: work already queued on the old stream must
         // finish before work on the new stream may reuse them
@@ -797,6 +798,13 @@ extern "C" int ude_set_stream(ude_ctx* c, void* s) {
         }
         c->stream = ns;
     }
+    return UDE_OK;
+}
+
+extern "C" int ude_set_operator_stream(ude_ctx* c, void* s) {
+    if (!c) return UDE_ERR_INVALID;
+    c->op_stream = (hipStream_t)s;
+    c->op_bound = true;
     return UDE_OK;
 }
 

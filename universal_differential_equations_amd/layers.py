@@ -4,7 +4,8 @@
 
 forward and pullback as single calls of libudecore's matrix-core kernels on torch CUDA tensors.  Rows of x are samples (the ABI's columns:
 a row-major (T, D) tensor IS the column-major D x T matrix); a weight is an (out, in) tensor held by rows (torch.nn.Linear's order) or by
-columns (`vec(W)` of Flux / Lux: W = torch.empty(n_in, n_out).T), all three in the same order.
+columns (`vec(W)` of Flux / Lux: W = torch.empty(n_in, n_out).T), all three in the same order.  Calls enqueue on torch's current stream and
+wait for no other: what was made on another stream is waited for by the caller, as everywhere in torch.
 """
 import ctypes as C
 
@@ -93,9 +94,9 @@ class _Block:
         return self.torch.empty(max(n.value, 256), dtype=self.torch.uint8, device=self.device), n.value
 
     def bind(self):
-        """this thread's context, on the current stream"""
+        """this thread's context, its operators on the current stream"""
         eng, stream = self.eng, current_raw_stream(self.device.index)
-        eng.set_stream(stream)
+        eng.set_operator_stream(stream)
         if stream != self.stream:
             # held since the forward call, on its stream; of x's copy (see _rows) and of gate and up nobody else has a reference: the memory is not
             # given away before this stream is done with it

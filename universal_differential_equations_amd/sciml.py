@@ -136,6 +136,10 @@ class Engine:
     def set_stream(self, stream_ptr):
         self.check(self.L.ude_set_stream(self.h, C.c_void_p(stream_ptr)))
 
+    def set_operator_stream(self, stream_ptr):
+        """of the training operators alone: they share no memory with the context's other calls, and wait for none of them"""
+        self.check(self.L.ude_set_operator_stream(self.h, stream_ptr))
+
     def kernel_ms(self):
         f, b = C.c_float(0), C.c_float(0)
         self.check(self.L.ude_last_kernel_ms(self.h, C.byref(f), C.byref(b)))

@@ -71,7 +71,7 @@ def _device_list(what, tensors):
 
 def _bound_engine(dev):
     eng = Engine.get(dev.index)
-    eng.set_stream(current_raw_stream(dev.index))
+    eng.set_operator_stream(current_raw_stream(dev.index))
     return eng
 
 
