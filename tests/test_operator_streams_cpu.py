@@ -118,3 +118,25 @@ assert eng.L.ude_set_operator_stream(eng.h, C.c_void_p(S)) == 0; assert go() == 
 eng.set_stream(A); assert go() == A
 assert eng.L.ude_set_operator_stream(None, None) == -1
 """)
+
+
+def test_the_current_device_stays(fake):
+    """operators on device 1, the first of which makes that device's context, while device 0 is the current one"""
+    run(fake, """
+assert fake.fake_device() == 0
+forward(block(device=1)); got = log(); assert {l for l in got} == {("launch", A, 1)}, got
+assert fake.fake_device() == 0
+at["stream"] = S
+forward(block(device=1, stream=S))
+assert fake.fake_device() == 0
+""")
+
+
+def test_the_current_device_stays_in_the_optimiser(fake):
+    run(fake, """
+training._bound_engine(types.SimpleNamespace(index=1))
+assert fake.fake_device() == 0
+at["stream"] = S
+training._bound_engine(types.SimpleNamespace(index=1))
+assert fake.fake_device() == 0
+""")

@@ -83,7 +83,7 @@ class _Block:
 
     @property
     def eng(self):
-        return Engine.get(self.device.index)
+        return Engine.get(self.device.index, keep_current=True)
 
     def workspace(self, pullback):
         n = C.c_int64(0)

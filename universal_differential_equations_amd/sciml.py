@@ -97,13 +97,16 @@ class Engine:
         self.device = device
 
     @classmethod
-    def get(cls, device=0):
-        """one context per (device, host thread), as include/udecore.h requires"""
+    def get(cls, device=0, keep_current=False):
+        """one context per (device, host thread), as include/udecore.h requires.  Making one leaves its device the current one; keep_current=True
+        (the training operators: nothing of theirs does) puts the old one back"""
+        import contextlib
         import threading
         key = (device, threading.get_ident())
         with cls._lock:
             if key not in cls._by_device:
-                cls._by_device[key] = Engine(device)
+                with __import__("torch").cuda.device(device) if keep_current else contextlib.nullcontext():
+                    cls._by_device[key] = Engine(device)
             return cls._by_device[key]
 
     def close(self):

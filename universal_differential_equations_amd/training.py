@@ -70,7 +70,7 @@ def _device_list(what, tensors):
 
 
 def _bound_engine(dev):
-    eng = Engine.get(dev.index)
+    eng = Engine.get(dev.index, keep_current=True)
     eng.set_operator_stream(current_raw_stream(dev.index))
     return eng
 
