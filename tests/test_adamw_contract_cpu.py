@@ -12,7 +12,7 @@ def training(monkeypatch):
     """the module, whose device checks take CPU tensors and whose launches append what they are given to `training.launched`: one dict of
     (grad as floats in the parameter's order, n) per tensor, and the step number"""
     from universal_differential_equations_amd import _lib, training
-    launched = []
+    launched, recorded = [], []
 
     def launch(handle, o, n, table):
         grads = []
@@ -25,11 +25,14 @@ def training(monkeypatch):
     def check(rc):
         assert rc == 0
 
-    eng = types.SimpleNamespace(h=None, check=check, L=types.SimpleNamespace(ude_adamw_step_dev=launch))
+    eng = types.SimpleNamespace(h=None, check=check, operator_stream=7, L=types.SimpleNamespace(ude_adamw_step_dev=launch))
     monkeypatch.setattr(training, "_device_list", lambda what, ts: (ts[0].device, str(ts[0].dtype)[6:]))
     monkeypatch.setattr(training, "_bound_engine", lambda dev: eng)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: "stream %d" % eng.operator_stream)
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, stream: recorded.append((t.data_ptr(), stream)))
     monkeypatch.setattr(training, "launched", launched, raising=False)
+    monkeypatch.setattr(training, "recorded", recorded, raising=False)
     assert _lib.ADAMW_BLOCK == 256
     return training
 
@@ -132,3 +135,24 @@ def test_parameter_arrays_of_the_deep_bsde_networks():
         assert len(sizes) == 14 and sum(sizes) == theta.size == sum(nets.num_params()) and sum(sizes[:6]) == nets.num_params()[0]
         for i, part in enumerate(np.split(theta, np.cumsum(sizes)[:-1])):
             assert part.any() == (i % 2 == 0)
+
+
+def test_states_are_kept_for_every_stream_that_steps(training):
+    """moments, scales, copies and the count are the instance's own: where it is dropped while a step is pending on another stream than they were
+    made on, their memory is not given away before"""
+    for kw in (dict(bits=32), dict(bits=8, capturable=True), dict(bits=32, master=True)):
+        p, q = (torch.zeros(600, dtype=torch.bfloat16 if "master" in kw else torch.float32) for _ in range(2))
+        opt = training.AdamW([p, q], **kw)
+        own = sorted(t.data_ptr() for t in [x for s in opt.state for x in s.values()] + ([opt.count] if kw.get("capturable") else []))
+        eng = training._bound_engine(None)
+        del training.recorded[:]
+        for eng.operator_stream in (7, 9, 9, 7):
+            opt.step([None, None])
+        assert sorted(x for x, stream in training.recorded if stream == "stream 9") == own
+        assert len(training.recorded) == 2 * len(own)    # (once a stream)
+        if opt.bits == 8:
+            eng.L.ude_adamw_moments_dev = lambda *a: 0
+            eng.operator_stream = 11
+            opt.moments()
+            assert sorted(x for x, stream in training.recorded if stream == "stream 11") == own
+        eng.operator_stream = 7

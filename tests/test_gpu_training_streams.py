@@ -108,3 +108,29 @@ def test_forward_calls_of_two_threads_are_all_compared():
     [t.start() for t in ts]
     [t.join() for t in ts]
     assert not bad and len(good) == 40
+
+
+@pytest.mark.parametrize("kw", [dict(bits=32), dict(bits=8, capturable=True), dict(bits=32, master=True)], ids=["32", "8", "copies"])
+def test_adamw_dropped_while_its_step_is_pending_on_another_stream(kw):
+    """its states' memory is not given to new work of the stream that made them: the step would write into that"""
+    from universal_differential_equations_amd import training
+    kind = torch.bfloat16 if kw.get("master") else torch.float32
+    n = 30000
+    start, g = torch.linspace(-1, 1, n, device="cuda").to(kind), torch.ones(n, dtype=kind, device="cuda")
+    p = start.clone()
+    training.AdamW([p], **kw).step([g])
+    want = p.clone()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        p.copy_(start)
+        opt = training.AdamW([p], **kw)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            occupy()
+            opt.step([g])
+        del opt
+        held = [torch.full((k,), 3, dtype=dt, device="cuda") for dt, k in ((torch.float32, n), (torch.int8, n), (torch.uint8, n), (torch.float32, -(-n // 256)), (torch.int64, 1))
+                for _ in range(6)]
+        torch.cuda.synchronize()
+        assert torch.equal(p, want) and all(bool((t == 3).all()) for t in held)
+        del held

@@ -142,6 +142,7 @@ class Engine:
     def set_operator_stream(self, stream_ptr):
         """of the training operators alone: they share no memory with the context's other calls, and wait for none of them"""
         self.check(self.L.ude_set_operator_stream(self.h, stream_ptr))
+        self.operator_stream = stream_ptr
 
     def kernel_ms(self):
         f, b = C.c_float(0), C.c_float(0)

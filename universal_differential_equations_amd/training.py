@@ -139,6 +139,7 @@ class AdamW:
         self._table = (_lib.AdamwTensor * n)()
         self._columns = np.frombuffer(self._table, dtype=np.int64).reshape(n, -1)   # the same memory; column 0: param, 1: grad, 7: n
         self._live = [0] * n
+        self._streams = set()   # those that the states are kept for
         for i, p in enumerate(self.params):
             s, t = self._state[i], self._table[i]
             t.master, t.m, t.v = (s[k].data_ptr() if k in s else None for k in ("master", "m", "v"))
@@ -228,7 +229,7 @@ class AdamW:
         o.clip = None if clip is None else clip.data_ptr()
         o.skip_nonfinite = int(self.skip_nonfinite)
         o.eta, (o.beta1, o.beta2), o.eps = self.eta, self.beta, self.eps
-        eng = _bound_engine(self.device)
+        eng = self._engine()
         if self.count is not None:
             self.count.add_(1)
             o.step_dev = self.count.data_ptr()
@@ -241,6 +242,18 @@ class AdamW:
         eng.check(rc)
         if self.count is None:
             self._steps += 1
+
+    def _engine(self):
+        """this thread's context on the current stream.  The states may have been made on another one: their memory is kept for this stream too, also
+        where the instance is dropped before its last step has run"""
+        eng = _bound_engine(self.device)
+        if eng.operator_stream not in self._streams:
+            now = self.torch.cuda.current_stream(self.device)
+            for t in (self.count, *(x for s in self._state for x in s.values())):
+                if t is not None:
+                    t.record_stream(now)
+            self._streams.add(eng.operator_stream)
+        return eng
 
     def _moved(self, at):
         """parameters were given other storage, or another layout of theirs"""
@@ -267,7 +280,7 @@ class AdamW:
                     raise ValueError("AdamW: output %d: float32 of %d elements on %s, contiguous, is needed" % (i, self._live[i], self.device))
         ms, vs = ((C.c_void_p * n)(*[pair[k].data_ptr() for pair in out]) for k in range(2))
         self._columns[:, 7] = self._live
-        eng = _bound_engine(self.device)
+        eng = self._engine()
         eng.check(eng.L.ude_adamw_moments_dev(eng.h, n, self._table, ms, vs))
         return out
 
