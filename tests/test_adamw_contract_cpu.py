@@ -156,3 +156,21 @@ def test_states_are_kept_for_every_stream_that_steps(training):
             opt.moments()
             assert sorted(x for x, stream in training.recorded if stream == "stream 11") == own
         eng.operator_stream = 7
+
+
+def test_parameters_that_were_given_shared_storage_are_refused(training):
+    """two chunks of a launch would update the same element at once"""
+    store = torch.zeros(20)
+    p, q = torch.zeros(8), torch.zeros(8)
+    opt = training.AdamW([p, q])
+    for other in (p.data, store[4:12]):
+        p.data = store[:8] if other is not p.data else p.data
+        q.data = other
+        with pytest.raises(ValueError, match="share"):
+            opt.step([torch.ones(8)] * 2)
+    q.data = opt.state[0]["m"]
+    with pytest.raises(ValueError, match="share"):
+        opt.step([torch.ones(8)] * 2)
+    q.data = store[8:16]
+    opt.step([torch.ones(8)] * 2)
+    assert opt.steps == 1 and len(training.launched) == 1

@@ -131,11 +131,7 @@ class AdamW:
         if state is not None and len(state) != n:
             raise ValueError("AdamW: state of %d tensors for %d parameters" % (len(state), n))
         self._state = [self._make_state(i, master, None if state is None else state[i]) for i in range(n)]
-        used = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), i) for i, p in enumerate(self.params)
-                      for t in (p, *self._state[i].values()) if t.numel())
-        for (_, end, i), (start, _, j) in zip(used, used[1:]):
-            if start < end:
-                raise ValueError("AdamW: parameters %d and %d, or their states, share memory" % (min(i, j), max(i, j)))
+        self._check_overlaps()
         self._table = (_lib.AdamwTensor * n)()
         self._columns = np.frombuffer(self._table, dtype=np.int64).reshape(n, -1)   # the same memory; column 0: param, 1: grad, 7: n
         self._live = [0] * n
@@ -171,6 +167,13 @@ class AdamW:
             if x.dtype != t or x.numel() != size or x.device != self.device or not x.is_contiguous():
                 raise ValueError("AdamW: state %d, %s: %s of %d elements on %s, contiguous, is needed" % (i, k, t, size, self.device))
         return dict(given)
+
+    def _check_overlaps(self):
+        used = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), i) for i, p in enumerate(self.params)
+                      for t in (p, *self._state[i].values()) if t.numel())
+        for (_, end, i), (start, _, j) in zip(used, used[1:]):
+            if start < end:
+                raise ValueError("AdamW: parameters %d and %d, or their states, share memory" % (min(i, j), max(i, j)))
 
     @property
     def state(self):
@@ -260,6 +263,7 @@ class AdamW:
         for i, p in enumerate(self.params):
             if p.device != self.device or str(p.dtype)[6:] != self.dtype or p.numel() != self._live[i] or not p.is_contiguous():
                 raise ValueError("AdamW: parameter %d was replaced by %s of %d elements on %s (strides %s)" % (i, p.dtype, p.numel(), p.device, p.stride()))
+        self._check_overlaps()
         self._columns[:, 0] = at
         self._at, self._shapes = at, [p.shape for p in self.params]
 
