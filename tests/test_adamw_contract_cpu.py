@@ -163,9 +163,8 @@ def test_parameters_that_were_given_shared_storage_are_refused(training):
     store = torch.zeros(20)
     p, q = torch.zeros(8), torch.zeros(8)
     opt = training.AdamW([p, q])
-    for other in (p.data, store[4:12]):
-        p.data = store[:8] if other is not p.data else p.data
-        q.data = other
+    for first, second in ((p.data, p.data), (store[:8], store[4:12])):
+        p.data, q.data = first, second
         with pytest.raises(ValueError, match="share"):
             opt.step([torch.ones(8)] * 2)
     q.data = opt.state[0]["m"]
