@@ -173,3 +173,14 @@ def test_parameters_that_were_given_shared_storage_are_refused(training):
     q.data = store[8:16]
     opt.step([torch.ones(8)] * 2)
     assert opt.steps == 1 and len(training.launched) == 1
+
+
+@pytest.mark.parametrize("most", [0, 0.0, -1.0, float("nan")])
+def test_a_norm_to_scale_to_is_positive(most):
+    """0 would scale to nothing on the host and not at all on the device (where grad_norm takes it for `no limit`)"""
+    import numpy as np
+    from universal_differential_equations_amd import pde, training as T
+    with pytest.raises(ValueError, match="max_norm"):
+        T.adamw(lambda th: (float(th @ th), 2 * th), np.ones(3), maxiters=2, max_norm=most)
+    with pytest.raises(ValueError, match="max_norm"):
+        pde.ADAMW(0.01, max_norm=most)

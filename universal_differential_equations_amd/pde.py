@@ -65,6 +65,8 @@ class ADAMW:
     def __init__(self, eta=0.001, beta=(0.9, 0.999), decay=0.0, max_norm=None):
         if not eta > 0:
             raise ValueError("ADAMW: eta = %r" % (eta,))
+        if max_norm is not None and not max_norm > 0:
+            raise ValueError("ADAMW: max_norm = %r" % (max_norm,))
         self.eta, self.beta, self.decay, self.max_norm, self.eps = eta, beta, decay, max_norm, 1e-8
 
 

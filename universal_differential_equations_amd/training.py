@@ -291,7 +291,9 @@ class AdamW:
 
 def adamw(loss_grad, theta, eta=0.001, beta=(0.9, 0.999), decay=0.01, maxiters=200, callback=None, eps=1e-8, max_norm=None, result="updated"):
     """`adam` with decoupled weight decay (theta <- theta (1 - eta decay) - ...) and, with max_norm, the gradient scaled to that norm where
-    it is larger.  theta: numpy, or a torch tensor; a CUDA tensor is updated by the fused step and stays on the device."""
+    it is larger (positive; None: no limit).  theta: numpy, or a torch tensor; a CUDA tensor is updated by the fused step and stays on the device."""
+    if max_norm is not None and not max_norm > 0:
+        raise ValueError("adamw: max_norm = %r" % (max_norm,))
     xp = _xp(theta)
     cuda = xp is not np and theta.is_cuda
     theta = theta.detach().clone(memory_format=xp.contiguous_format) if xp is not np else np.array(theta, dtype=np.float64)
