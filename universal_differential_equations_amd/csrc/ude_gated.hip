@@ -31,6 +31,8 @@ int check(ude_ctx* c, const ude_gated_ffn_desc* d) {
     const int64_t most = INT32_MAX - 1024;
     if (d->T < 0 || d->D < 1 || d->F < 1 || d->O < 1 || d->T > most || d->D > most || d->F > most / 2 || d->O > most)
         return fail(c, UDE_ERR_INVALID, "gated_ffn: sizes T = %lld, D = %lld, F = %lld, O = %lld", (long long)d->T, (long long)d->D, (long long)d->F, (long long)d->O);
+    if (d->T * d->F > (int64_t)1 << 58)  // (three such matrices of four bytes an element: the workspace's size has to fit 64 bits)
+        return fail(c, UDE_ERR_UNSUPPORTED, "gated_ffn: a hidden layer of T x F = %lld x %lld", (long long)d->T, (long long)d->F);
     const int64_t gcols = d->w_order ? d->D : d->F, dcols = d->w_order ? d->F : d->O;
     if (d->ldx < d->D || d->ldy < d->O || d->ldg < gcols || d->ldu < gcols || d->ldd < dcols || d->ldx > most || d->ldy > most || d->ldg > most || d->ldu > most || d->ldd > most)
         return fail(c, UDE_ERR_INVALID, "gated_ffn: a leading dimension is smaller than what it spans, or over 2^31");
@@ -148,8 +150,8 @@ bool few(const Args& a, int epi, int es, bool tile) {
 }
 // no product of these sizes, nor some of `n` such products side by side, leaves more bytes of parts than this
 int64_t part_bytes(int64_t M, int64_t N, int64_t steps, int n) {
-    const int64_t all = n * ((M + 127) / 128) * ((N + 63) / 64) * (steps / 2);  // (part bytes of a tile go with its area: the largest tile's)
-    return all < MOST_PART_BYTES / 65536 ? all * 65536 : MOST_PART_BYTES;
+    const double all = (double)n * ((M + 127) / 128) * ((N + 63) / 64) * (steps / 2);  // (exact where it counts; part bytes of a tile go with its area: the largest tile's)
+    return all < MOST_PART_BYTES / 65536 ? (int64_t)all * 65536 : MOST_PART_BYTES;
 }
 
 // a row starts on a 4-byte boundary, and a tile's offsets fit 31 bits
