@@ -344,7 +344,8 @@ enum { UDE_GATE_IDENTITY = 0, UDE_GATE_TANH = 1, UDE_GATE_RBF = 2 /* exp(-x^2) *
        UDE_GATE_SWISH = 5 /* x sigmoid(x) */, UDE_GATE_GELU_TANH = 6, UDE_GATE_GELU_ERF = 7 };
 /* y = (act(Wg x) .* (Wu x)) -> Wd, column by column:  y_j = Wd (act(Wg x_j) .* (Wu x_j)),  x: D x T, Wg, Wu: F x D, Wd: O x F, y: O x T
  * column-major (column j = sample / token j).  Products are summed in Float32 and act is evaluated in Float32 for every dtype; act(..) .*
- * (..) and, in the pullback, the two cotangents of the hidden layer are rounded to dtype where they enter the next product. */
+ * (..) and, in the pullback, the two cotangents of the hidden layer are rounded to dtype where they enter the next product: in Float16 they are
+ * infinite from 65520 on and zero below 2^-25 (scale the loss: the pullback is linear in dy). */
 typedef struct {
     int32_t dtype;    /* UDE_DT_F32 / F16 / BF16: x, weights, y, cotangents, gradients */
     int32_t act;      /* UDE_GATE_* */

@@ -7,6 +7,9 @@
 //              dWg = dg^T x, dWu = du^T x, dWd = dy^T h
 // Rows are samples (x: T x D row-major = the ABI's D x T column-major).  Every product is C[m, n] = sum_k A(m, k) B(n, k) with each
 // operand stored either with consecutive k adjacent ("K") or with consecutive rows adjacent ("R"): that covers both weight orders.
+// h, dg and du are rounded to the block's type, because an operand of a 16-bit matrix instruction has 16 bits: the error of y against Float64 is
+// sqrt 2 of one rounding's (0.0024 of its norm in BFloat16, 0.00029 in Float16, against 0.0017 and 0.0002 with h in Float32).  h as the sum of two 16-bit
+// values would take that back for twice the instructions of every product that it enters: a third more for the forward call, five sixths (with dg and du) for the pullback.
 #pragma once
 #include <hip/hip_runtime.h>
 

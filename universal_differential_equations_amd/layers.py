@@ -126,7 +126,9 @@ def gated_ffn(x, w_gate, w_up, w_down, act="swish", save=False):
     """y = Wd (act(Wg x) .* (Wu x)) for every row of x (..., D); w_gate, w_up: (F, D), w_down: (O, F).  act: identity, tanh, rbf, relu,
     sigmoid, swish, gelu_tanh or gelu_erf.  save=True returns (y, saved) for `gated_ffn_pullback`: `saved` holds references to x and the
     weights -- change them in place only after the pullback -- and Wg x, Wu x in Float32.  No autograd graph is recorded: the pullback is the
-    gradient.  Rounding: sums and act in Float32; act(..) .* (..) is rounded to x's dtype once, where it enters the last product."""
+    gradient.  Rounding: sums and act in Float32; act(..) .* (..) is rounded to x's dtype once, where it enters the last product, and so are its
+    two cotangents in the pullback.  With float16 that is a matter of range too: a hidden value from 65520 on is infinite, also where y would not be, and
+    a hidden cotangent under 3e-8 is zero, with its share of the gradients -- scale the loss (the pullback is linear in dy), or take bfloat16."""
     b = _Block(x, w_gate, w_up, w_down, act)
     torch, D = b.torch, b.D
     t, f, o = D.T, D.F, D.O
