@@ -36,7 +36,7 @@ class Device:                        # torch.cuda.device
         fake.hipSetDevice(self.d)
     def __exit__(self, *a):
         fake.hipSetDevice(self.old)
-cuda = types.SimpleNamespace(current_stream=lambda d: at["stream"], device=Device)
+cuda = types.SimpleNamespace(current_stream=lambda d: at["stream"], device=Device, is_current_stream_capturing=lambda: False)
 sys.modules["torch"] = types.SimpleNamespace(cuda=cuda)
 def block(device=0, stream=A):
     b = layers._Block.__new__(layers._Block)
@@ -139,4 +139,23 @@ assert fake.fake_device() == 0
 at["stream"] = S
 training._bound_engine(types.SimpleNamespace(index=1))
 assert fake.fake_device() == 0
+""")
+
+
+def test_the_first_call_of_a_thread_inside_a_capture_is_refused(fake):
+    """it would make the thread's context, whose allocations end a capture; afterwards, and with a context there, captures are taken"""
+    run(fake, """
+cuda.is_current_stream_capturing = lambda: True
+for go in (lambda: block().bind(), lambda: training._bound_engine(types.SimpleNamespace(index=0))):
+    try:
+        go()
+        assert False, "not refused"
+    except ValueError as e:
+        assert "captured" in str(e)
+assert not sciml.Engine._by_device and not log()
+cuda.is_current_stream_capturing = lambda: False
+block().bind()
+cuda.is_current_stream_capturing = lambda: True
+fake.fake_capture(A)
+forward(block()); got = log(); assert {l[:2] for l in got} == {("launch", A)}, got
 """)

@@ -100,14 +100,20 @@ class Engine:
     def get(cls, device=0, keep_current=False):
         """one context per (device, host thread), as include/udecore.h requires.  Making one leaves its device the current one; keep_current=True
         (the training operators: nothing of theirs does) puts the old one back"""
-        import contextlib
         import threading
         key = (device, threading.get_ident())
         with cls._lock:
             if key not in cls._by_device:
-                with __import__("torch").cuda.device(device) if keep_current else contextlib.nullcontext():
-                    cls._by_device[key] = Engine(device)
+                cls._by_device[key] = cls._keeping_current(device) if keep_current else Engine(device)
             return cls._by_device[key]
+
+    @classmethod
+    def _keeping_current(cls, device):
+        import torch
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError("the first call of a thread makes its context, which cannot be captured into a graph: call once before")
+        with torch.cuda.device(device):
+            return cls(device)
 
     def close(self):
         if self.h is not None:
