@@ -184,3 +184,20 @@ def test_a_norm_to_scale_to_is_positive(most):
         T.adamw(lambda th: (float(th @ th), 2 * th), np.ones(3), maxiters=2, max_norm=most)
     with pytest.raises(ValueError, match="max_norm"):
         pde.ADAMW(0.01, max_norm=most)
+
+
+def test_steps_with_and_without_some_gradients_in_turn(training):
+    """the table that is kept between steps: which tensors a launch leaves out is decided by that step's gradients alone"""
+    ps = [torch.zeros(4), torch.zeros(5), torch.zeros(6)]
+    opt = training.AdamW(ps, bits=8)
+    training._bound_engine(None).L.ude_adamw_moments_dev = lambda *a: 0
+    gs = [torch.full((k,), float(k)) for k in (4, 5, 6)]
+    want = []
+    for keep in ((1, 1, 1), (1, 0, 1), (0, 0, 0), (1, 1, 1), (0, 1, 0), (0, 1, 1), (1, 1, 1), (1, 1, 1)):
+        given = [g if k else None for g, k in zip(gs, keep)]
+        opt.step(given)
+        want.append([None if g is None else g.tolist() for g in given])
+        opt.moments()
+        with pytest.raises(ValueError):
+            opt.step([None, gs[0], gs[2]])
+    assert [x.grads for x in training.launched] == want

@@ -12,6 +12,7 @@ device-resident ones on torch's current stream.  Arrays follow Julia's layout: a
 (n, ns) per trajectory, an ensemble solution (N, ns, n) in C order == n x ns x N column-major.
 """
 import ctypes as C
+import threading
 
 import numpy as np
 
@@ -85,7 +86,7 @@ class Engine:
     """One ude_ctx (device + stream).  Created lazily per device."""
 
     _by_device = {}
-    _lock = __import__("threading").Lock()
+    _lock = threading.Lock()
 
     def __init__(self, device=0):
         self.L = _lib.load()
@@ -100,7 +101,6 @@ class Engine:
     def get(cls, device=0, keep_current=False):
         """one context per (device, host thread), as include/udecore.h requires.  Making one leaves its device the current one; keep_current=True
         (the training operators: nothing of theirs does) puts the old one back"""
-        import threading
         key = (device, threading.get_ident())
         with cls._lock:
             if key not in cls._by_device:

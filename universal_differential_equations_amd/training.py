@@ -136,6 +136,7 @@ class AdamW:
         self._columns = np.frombuffer(self._table, dtype=np.int64).reshape(n, -1)   # the same memory; column 0: param, 1: grad, 7: n
         self._live = [0] * n
         self._streams = set()   # those that the states are kept for
+        self._partial = False   # the table's numbers of elements leave out tensors that had no gradient
         for i, p in enumerate(self.params):
             s, t = self._state[i], self._table[i]
             t.master, t.m, t.v = (s[k].data_ptr() if k in s else None for k in ("master", "m", "v"))
@@ -143,7 +144,8 @@ class AdamW:
             t.param, t.n, t.weight_decay = p.data_ptr(), p.numel(), decay[i]
             self._live[i] = p.numel()
         self._at, self._shapes = [p.data_ptr() for p in self.params], [p.shape for p in self.params]
-        self._opts = _lib.AdamwOpts(param_dtype=_lib.DTYPE_CODE[self.dtype], state_bits=bits)
+        self._opts = _lib.AdamwOpts(param_dtype=_lib.DTYPE_CODE[self.dtype], grad_dtype=_lib.DTYPE_CODE[self.dtype], state_bits=bits)
+        self._grad_dtype = None   # what grad_dtype was written for
 
     def _make_state(self, i, master, given):
         torch, p = self.torch, self.params[i]
@@ -221,12 +223,16 @@ class AdamW:
             grads = [g if g is None else g.contiguous() for g in grads]   # (kept until the launch)
         if len(have) == len(grads):
             self._columns[:, 1] = [g.data_ptr() for g in grads]
-            self._columns[:, 7] = self._live
+            if self._partial:
+                self._columns[:, 7] = self._live
         else:
             self._columns[:, 1] = [0 if g is None else g.data_ptr() for g in grads]
             self._columns[:, 7] = [0 if g is None else k for g, k in zip(grads, self._live)]
+        self._partial = len(have) < len(grads)
         o = self._opts
-        o.grad_dtype = _lib.DTYPE_CODE.get(str(dts.pop())[6:], -1) if dts else o.param_dtype
+        dt = dts.pop() if dts else None
+        if dt is not self._grad_dtype:
+            self._grad_dtype, o.grad_dtype = dt, o.param_dtype if dt is None else _lib.DTYPE_CODE.get(str(dt)[6:], -1)
         if clip is not None and (clip.dtype != torch.float64 or clip.numel() != 2 or clip.device != self.device or not clip.is_contiguous()):
             raise ValueError("AdamW: clip is what grad_norm returns: a float64 tensor [norm, factor] on %s" % self.device)
         o.clip = None if clip is None else clip.data_ptr()
@@ -283,7 +289,7 @@ class AdamW:
                 if x.dtype != torch.float32 or x.numel() != self._live[i] or x.device != self.device or not x.is_contiguous():
                     raise ValueError("AdamW: output %d: float32 of %d elements on %s, contiguous, is needed" % (i, self._live[i], self.device))
         ms, vs = ((C.c_void_p * n)(*[pair[k].data_ptr() for pair in out]) for k in range(2))
-        self._columns[:, 7] = self._live
+        self._columns[:, 7], self._partial = self._live, False
         eng = self._engine()
         eng.check(eng.L.ude_adamw_moments_dev(eng.h, n, self._table, ms, vs))
         return out
