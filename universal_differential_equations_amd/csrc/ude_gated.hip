@@ -45,7 +45,8 @@ int vec(const void* p, int64_t ld, int e) { return (uintptr_t)p % 16 == 0 && ld 
 
 // Tiles on the 256 compute units of an MI355X: microseconds that a step of 128 bytes of k takes with 1, 2, 3 workgroups on a compute unit, and
 // the start and epilogue of a round, as measured (kernel times over products of 64 x 512 x 1408 to 4096 x 4096 x 11264).
-//   256 x 256: the least that is read again: 4096 x 4096 x 11264 in 271 us = 1395 TFLOP/s; 256 x 128: 311 us; 128 x 128: 365 us.
+//   256 x 256: the least that is read again: 4096 x 4096 x 11264 in 279 us at best and 298 in the median of a profiled run (1355 and 1268 TFLOP/s: the
+//   card's clock); in the run that these times were fitted to 271, with 256 x 128 311 and with 128 x 128 365.
 //   The smaller ones leave less of the last round idle, but a step costs them 0.25 to 0.5 however little there is in it (LDS, barrier, the
 //   loads' way: 64 x 64 takes 0.28 with its loads four steps ahead, 0.41 with two), so that they are for small products, and for Float32, whose matrix instructions (1/16 of the 16-bit rate) bound it with
 //   any tile.

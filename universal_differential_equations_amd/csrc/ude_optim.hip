@@ -248,7 +248,7 @@ __device__ inline int row_max(int x) {
 
 // 16 lanes hold one block of 256 elements, 8 consecutive ones of each half, so that the 16-byte accesses of 16-bit parameters lie side by
 // side.  Bound by its arithmetic: 88 vector instructions an element, 30 of them Float64, five roots and reciprocals at a quarter of the rate.  138.4 M
-// elements in BFloat16 take 355 us where their 10 bytes each would take 245 at the rate of the Float32 moments' step (with correctly rounded
+// elements in BFloat16 take 353 us (launches in a row; 377 to 509 alone, where the clock rises first) where their 10 bytes each would take 245 at the rate of the Float32 moments' step (with correctly rounded
 // root and quotient, 108 instructions: 430).  Deciding the codes in Float32 where they are clear took longer: the branches cost more.
 template <class P, class G>
 __global__ __launch_bounds__(256) void adamw8_kernel(const AdamArgs a) {
