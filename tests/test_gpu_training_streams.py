@@ -134,3 +134,29 @@ def test_adamw_dropped_while_its_step_is_pending_on_another_stream(kw):
         torch.cuda.synchronize()
         assert torch.equal(p, want) and all(bool((t == 3).all()) for t in held)
         del held
+
+
+def test_captured_pullback_of_an_eager_forward():
+    """the forward call on the main stream, its pullback captured on another and replayed three times with other cotangents and eager work between; what
+    was saved is dropped in the end, and the memory is used again"""
+    import universal_differential_equations_amd as U
+    T, D, F, O = 150, 72, 104, 40
+    xt, wg, wu, wd, dy = made(T, D, F, O, torch.bfloat16, 26)
+    dys = [dy * k for k in (1.0, -2.0, 0.5)]
+    want = [U.gated_ffn_pullback(U.gated_ffn(xt.T, wg, wu, wd, save=True)[1], d) for d in dys]
+    saved = U.gated_ffn(xt.T, wg, wu, wd, save=True)[1]
+    held = dy.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = U.gated_ffn_pullback(saved, held)
+    for d, w in zip(dys, want):
+        held.copy_(d)
+        graph.replay()
+        again = U.gated_ffn_pullback(saved, d)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(got, w, again))
+    del graph, got, saved
+    held = fill_with_nan([(T, D), (2, T, F)], torch.bfloat16)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want[0], U.gated_ffn_pullback(U.gated_ffn(xt.T, wg, wu, wd, save=True)[1], dys[0])))

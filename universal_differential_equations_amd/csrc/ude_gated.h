@@ -731,7 +731,8 @@ __global__ __launch_bounds__(64 * NWM * NWN) void join_parts(const Args a) {
 // C[m, n] = sum_k A(m, k) B(n, k) for at most ROWS rows of A where B's k are adjacent: a wavefront for NB rows of B (EPI_GATE: half of them of Wg, half
 // of Wu), 16 bytes of k a lane, sums in Float32 over the lanes at the end.  Bound by reading B, once and in full lines: a tile of matrix instructions
 // does that too, but has to cut K to fill the card and join the parts in launches of their own.  One row through a block of 4096 x 11264 in
-// BFloat16 takes 44.5 us = 6.2 TB/s (32 x 128 tiles: 67), four rows 68 (68), in Float32 116 (139); through 2048 x 5632 18 us (31) and 26 (31).  With more
+// BFloat16 takes 44 us = 6.3 TB/s (32 x 128 tiles: 67 to 75), four rows 64 to 66 (67 to 75), one row in Float32 84 = 6.6 TB/s (118); through 2048 x 5632 15 to 17 us
+// (27 to 32) and 25 (27 to 32): the same weights again, and six sets of them in turn.  With more
 // rows the loads of A and the conversions outweigh those of B (eight rows: 150 us): four rows of B a wavefront instead of two took two
 // rows from 64 to 57 us and four from 89 to 68.
 template <int EPI, int ROWS>
