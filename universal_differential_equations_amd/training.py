@@ -105,7 +105,8 @@ class AdamW:
     are used as they are, e.g. another instance's `state` out of a checkpoint; step: the steps already done.  capturable=True counts
     the steps on the device (`count`, which `steps` reads), as a step that is captured into a hipGraph needs; eta, beta, eps and decay are those of the
     capture.  skip_nonfinite=True leaves everything as it was in a step
-    whose clip[0] is not finite (the step is counted).  A non-finite gradient makes the 8-bit moments of its block of 256 NaN."""
+    whose clip[0] is not finite (the step is counted).  A non-finite gradient makes the 8-bit moments of its block of 256 NaN, and so does one whose
+    square's share of v passes Float32.  A step enqueues on torch's current stream: where steps are on several, the caller orders them."""
 
     def __init__(self, params, eta=0.001, beta=(0.9, 0.999), eps=1e-8, weight_decay=0.01, bits=32, master=False, state=None, step=0,
                  skip_nonfinite=False, capturable=False):
